@@ -23,6 +23,7 @@ QKV_EDEVICE = -6
 
 QKV_BF16, QKV_F16, QKV_F32 = 0, 1, 2
 QKV_MASK_NONE, QKV_MASK_CAUSAL, QKV_MASK_BOOL, QKV_MASK_ADDITIVE = 0, 1, 2, 3
+QKV_ACT_NONE, QKV_ACT_SWIGLU = 0, 1
 QKV_OUT_NORMALIZED, QKV_OUT_PARTIAL = 0, 1
 QKV_IPC_HANDLE_BYTES = 64  # size of a CUDA IPC memory handle (qkv_peer_alloc)
 
@@ -77,6 +78,26 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
          _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp],
     ),
+    "qkv_matmul_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "qkv_quantized_matmul": (
+        _i,
+        [_vp, _ll, _vp, _vp, _vp, _vp,  # x ldx w scales biases out
+         _i, _i, _i, _i, _i, _i, _i,  # M N K bits group_size dtype act
+         _vp, _sz, _vp],  # workspace ws_bytes stream
+    ),
+    "qkv_grouped_matmul": (
+        _i,
+        [_vp, _ll, _i, _vp, _vp, _vp, _vp, _vp, _vp,  # x ldx x_rows rows offsets w s b out
+         _i, _i, _i, _i, _i, _i, _i, _i,  # R E N K bits group_size dtype act
+         _vp, _sz, _vp],  # workspace ws_bytes stream
+    ),
+    "qkv_route_workspace_size": (_sz, [_i, _i]),
+    "qkv_route_topk": (
+        _i,
+        [_vp, _i, _i, _i, _i, _i,  # logits dtype T E k normalize
+         _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],  # experts weights rows slots offsets ws
+    ),
+    "qkv_expert_combine": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
 }
 
 _lib = None
@@ -85,7 +106,9 @@ _lock = threading.Lock()
 # entry points with CPython bindings (chad_b200._qkvext): the per-layer calls
 EXT_BOUND = {"qkv_attention": "attention", "qkv_prefill": "prefill",
              "qkv_quantize_append_kv": "quantize_append_kv", "qkv_combine": "combine",
-             "qkv_gather_combine": "gather_combine"}
+             "qkv_gather_combine": "gather_combine",
+             "qkv_quantized_matmul": "quantized_matmul", "qkv_grouped_matmul": "grouped_matmul",
+             "qkv_route_topk": "route_topk", "qkv_expert_combine": "expert_combine"}
 
 
 class QKVError(RuntimeError):

@@ -1,0 +1,49 @@
+// Launch interface of the 4-bit weight products (qkv_matmul.cu, qkv_matmul_tc.cu) and of the
+// expert routing around them (qkv_experts.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+namespace qkv {
+
+// One product y[r] = act(x[rows[r]] W_e^T) over the rows r of every expert e
+// (offsets[e] <= r < offsets[e+1]); without offsets one weight matrix and all R rows.
+struct MatmulArgs {
+  const void* x;       // (x_rows, K) in dtype, ldx elements between rows
+  long long ldx;
+  int x_rows;          // rows of x; an entry of `rows` outside [0, x_rows) reads as zeros
+  const int* rows;     // device int32[R] or nullptr (row r of y comes from row r of x)
+  const int* offsets;  // device int32[E + 1] or nullptr
+  const void* w;       // codes (E, N, K/8) uint32
+  const void* scales;  // (E, N, K/64) in dtype
+  const void* biases;
+  void* out;           // (R, N) in dtype, (R, N/2) with the gated activation
+  int R, E, N, K;
+  int dtype;           // QKV_BF16 / QKV_F16
+  int act;             // QKV_ACT_NONE / QKV_ACT_SWIGLU
+  void* workspace;
+  size_t ws_bytes;
+  int* status;         // device status word for bounded-wait failures
+};
+
+int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st);  // few rows per weight matrix
+
+struct RouteArgs {
+  const void* logits;  // (T, E) in dtype
+  int dtype, T, E, k, normalize;
+  int* experts;        // (T, k)
+  float* weights;      // (T, k)
+  int* rows;           // (T * k) token of each sorted pair
+  int* slots;          // (T, k) sorted position of each pair
+  int* offsets;        // (E + 1)
+  int* hist;           // workspace: (blocks, E)
+};
+
+size_t route_workspace_bytes(int T, int E);
+int launch_route(const RouteArgs& a, cudaStream_t st);
+int launch_expert_combine(const void* y, int R, const int* slots, const float* weights,
+                          const void* residual, void* out, int T, int k, int N, int dtype,
+                          cudaStream_t st);
+
+}  // namespace qkv

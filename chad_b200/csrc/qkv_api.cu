@@ -9,6 +9,7 @@
 #include <atomic>
 
 #include "../../include/qkv.h"
+#include "matmul_internal.h"
 #include "qkv_internal.h"
 
 
@@ -430,6 +431,149 @@ int qkv_prefill(const void* q, const void* k_new, const void* v_new, void* kw, v
   }
   if (rc) return fail(rc, "prefill: unsupported configuration");
   return cuda_check("qkv_prefill");
+}
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Validate and pack the shared arguments of the 4-bit weight products.
+int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const int* rows,
+                 const int* offsets, const void* w, const void* scales, const void* biases,
+                 void* out, int R, int E, int N, int K, int bits, int group_size, int dtype,
+                 int act, void* workspace, size_t ws_bytes) {
+  if (bits != 4) return fail(QKV_EUNSUPPORTED, "weights must have 4 bits (got %d)", bits);
+  if (group_size != 64)
+    return fail(QKV_EUNSUPPORTED, "group_size must be 64 (got %d)", group_size);
+  if (dtype != QKV_BF16 && dtype != QKV_F16) return fail(QKV_EINVAL, "bad dtype %d", dtype);
+  if (act != QKV_ACT_NONE && act != QKV_ACT_SWIGLU) return fail(QKV_EINVAL, "bad act %d", act);
+  if (R < 0 || x_rows < 0 || E <= 0 || N <= 0 || K <= 0)
+    return fail(QKV_EINVAL, "bad sizes R=%d x_rows=%d E=%d N=%d K=%d", R, x_rows, E, N, K);
+  if (K % 64) return fail(QKV_EINVAL, "K %d is not a multiple of 64", K);
+  if (act == QKV_ACT_SWIGLU && N % 2)
+    return fail(QKV_EINVAL, "N %d is odd: gate and up need as many rows", N);
+  if (ldx < K) return fail(QKV_EINVAL, "row stride %lld of x is below K %d", ldx, K);
+  if (R > 0) {
+    if (!x || !w || !scales || !biases || !out) return fail(QKV_EINVAL, "null tensor pointer");
+    if (!aligned16(x) || ldx % 8) return fail(QKV_EALIGN, "rows of x must be 16-byte aligned");
+    if (!aligned16(w)) return fail(QKV_EALIGN, "w must be 16-byte aligned");
+    if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(out, 2) || !aligned(rows, 4) ||
+        !aligned(offsets, 4))
+      return fail(QKV_EALIGN, "scales, biases, out, rows and offsets must be naturally aligned");
+  }
+  a = MatmulArgs{};
+  a.x = x;
+  a.ldx = ldx;
+  a.x_rows = x_rows;
+  a.rows = rows;
+  a.offsets = offsets;
+  a.w = w;
+  a.scales = scales;
+  a.biases = biases;
+  a.out = out;
+  a.R = R;
+  a.E = E;
+  a.N = N;
+  a.K = K;
+  a.dtype = dtype;
+  a.act = act;
+  const size_t need = qkv_matmul_workspace_size(R, E, N, K, dtype, act);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(QKV_EWORKSPACE, "workspace %zu bytes < required %zu", ws_bytes, need);
+  if (need && !aligned16(workspace)) return fail(QKV_EALIGN, "workspace must be 16-byte aligned");
+  a.workspace = workspace;
+  a.ws_bytes = ws_bytes;
+  a.status = status_ptr();
+  return QKV_OK;
+}
+
+}  // namespace
+
+size_t qkv_matmul_workspace_size(int M, int E, int N, int K, int dtype, int act) {
+  (void)M;
+  (void)E;
+  (void)N;
+  (void)K;
+  (void)dtype;
+  (void)act;
+  return 0;
+}
+
+int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void* scales,
+                         const void* biases, void* out, int M, int N, int K, int bits,
+                         int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
+                         void* stream) {
+  MatmulArgs a;
+  int rc = setup_matmul(a, x, ldx, M, nullptr, nullptr, w, scales, biases, out, M, 1, N, K, bits,
+                        group_size, dtype, act, workspace, ws_bytes);
+  if (rc || M == 0) return rc;
+  rc = launch_matmul_rows(a, static_cast<cudaStream_t>(stream));
+  if (rc) return fail(rc, "quantized_matmul: unsupported shape");
+  return cuda_check("qkv_quantized_matmul");
+}
+
+int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows,
+                       const int* offsets, const void* w, const void* scales,
+                       const void* biases, void* out, int R, int E, int N, int K, int bits,
+                       int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
+                       void* stream) {
+  if (R > 0 && !offsets) return fail(QKV_EINVAL, "null offsets");
+  if (!rows && R > x_rows) return fail(QKV_EINVAL, "R %d exceeds the %d rows of x", R, x_rows);
+  MatmulArgs a;
+  int rc = setup_matmul(a, x, ldx, x_rows, rows, offsets, w, scales, biases, out, R, E, N, K,
+                        bits, group_size, dtype, act, workspace, ws_bytes);
+  if (rc || R == 0) return rc;
+  rc = launch_matmul_rows(a, static_cast<cudaStream_t>(stream));
+  if (rc) return fail(rc, "grouped_matmul: unsupported shape");
+  return cuda_check("qkv_grouped_matmul");
+}
+
+size_t qkv_route_workspace_size(int T, int E) {
+  return T <= 0 || E <= 0 ? 0 : route_workspace_bytes(T, E);
+}
+
+int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int normalize,
+                   int* experts, float* weights, int* rows, int* slots, int* offsets,
+                   void* workspace, size_t ws_bytes, void* stream) {
+  if (dtype != QKV_BF16 && dtype != QKV_F16 && dtype != QKV_F32)
+    return fail(QKV_EINVAL, "bad dtype %d", dtype);
+  if (T < 0 || E <= 0 || k <= 0 || k > E)
+    return fail(QKV_EINVAL, "bad sizes T=%d E=%d k=%d", T, E, k);
+  if (E > 512 || k > 16)
+    return fail(QKV_EUNSUPPORTED, "at most 512 experts and 16 choices (got %d, %d)", E, k);
+  if ((long long)T * k > 0x7fffffffll)
+    return fail(QKV_EUNSUPPORTED, "T * k exceeds 32-bit positions (T=%d k=%d)", T, k);
+  if (!offsets || (T > 0 && (!logits || !experts || !weights || !rows || !slots)))
+    return fail(QKV_EINVAL, "null pointer");
+  if (!aligned(logits, dtype == QKV_F32 ? 4 : 2) || !aligned(experts, 4) ||
+      !aligned(weights, 4) || !aligned(rows, 4) || !aligned(slots, 4) || !aligned(offsets, 4))
+    return fail(QKV_EALIGN, "pointers must be naturally aligned");
+  const size_t need = qkv_route_workspace_size(T, E);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(QKV_EWORKSPACE, "workspace %zu bytes < required %zu", ws_bytes, need);
+  if (need && !aligned16(workspace)) return fail(QKV_EALIGN, "workspace must be 16-byte aligned");
+  const RouteArgs a = {logits, dtype, T, E, k, normalize, experts, weights, rows, slots, offsets,
+                       (int*)workspace};
+  const int rc = launch_route(a, static_cast<cudaStream_t>(stream));
+  if (rc) return fail(rc, "route: launch failed");
+  return cuda_check("qkv_route_topk");
+}
+
+int qkv_expert_combine(const void* y, int R, const int* slots, const float* weights,
+                       const void* residual, void* out, int T, int k, int N, int dtype,
+                       void* stream) {
+  if (dtype != QKV_BF16 && dtype != QKV_F16) return fail(QKV_EINVAL, "bad dtype %d", dtype);
+  if (R < 0 || T < 0 || k <= 0 || N <= 0)
+    return fail(QKV_EINVAL, "bad sizes R=%d T=%d k=%d N=%d", R, T, k, N);
+  if (T == 0) return QKV_OK;
+  if ((R > 0 && !y) || !slots || !weights || !out) return fail(QKV_EINVAL, "null pointer");
+  if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned(slots, 4) ||
+      !aligned(weights, 4))
+    return fail(QKV_EALIGN, "y, residual and out must be 16-byte aligned");
+  const int rc = launch_expert_combine(y, R, slots, weights, residual, out, T, k, N, dtype,
+                                       static_cast<cudaStream_t>(stream));
+  if (rc) return fail(rc, "expert_combine: unsupported shape");
+  return cuda_check("qkv_expert_combine");
 }
 
 }  // extern "C"

@@ -20,6 +20,10 @@ static __typeof__(&qkv_prefill) p_prefill;
 static __typeof__(&qkv_quantize_append_kv) p_append_kv;
 static __typeof__(&qkv_combine) p_combine;
 static __typeof__(&qkv_gather_combine) p_gather_combine;
+static __typeof__(&qkv_quantized_matmul) p_quantized_matmul;
+static __typeof__(&qkv_grouped_matmul) p_grouped_matmul;
+static __typeof__(&qkv_route_topk) p_route_topk;
+static __typeof__(&qkv_expert_combine) p_expert_combine;
 
 typedef union {
   void* p;
@@ -147,6 +151,50 @@ static PyObject* w_gather_combine(PyObject* self, PyObject* const* args, Py_ssiz
   return PyLong_FromLong(rc);
 }
 
+static PyObject* w_quantized_matmul(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  Arg a[16];
+  (void)self;
+  if (!p_quantized_matmul) return unbound("qkv_quantized_matmul"), NULL;
+  if (parse(args, n, "plpppp" "iiiiiii" "pzp", a)) return NULL;
+  const int rc = p_quantized_matmul(a[0].p, a[1].l, a[2].p, a[3].p, a[4].p, a[5].p, a[6].i,
+                                    a[7].i, a[8].i, a[9].i, a[10].i, a[11].i, a[12].i, a[13].p,
+                                    a[14].z, a[15].p);
+  return PyLong_FromLong(rc);
+}
+
+static PyObject* w_grouped_matmul(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  Arg a[20];
+  (void)self;
+  if (!p_grouped_matmul) return unbound("qkv_grouped_matmul"), NULL;
+  if (parse(args, n, "plipppppp" "iiiiiiii" "pzp", a)) return NULL;
+  const int rc = p_grouped_matmul(a[0].p, a[1].l, a[2].i, (const int*)a[3].p,
+                                  (const int*)a[4].p, a[5].p, a[6].p, a[7].p, a[8].p, a[9].i,
+                                  a[10].i, a[11].i, a[12].i, a[13].i, a[14].i, a[15].i, a[16].i,
+                                  a[17].p, a[18].z, a[19].p);
+  return PyLong_FromLong(rc);
+}
+
+static PyObject* w_route_topk(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  Arg a[14];
+  (void)self;
+  if (!p_route_topk) return unbound("qkv_route_topk"), NULL;
+  if (parse(args, n, "piiiii" "pppppp" "zp", a)) return NULL;
+  const int rc = p_route_topk(a[0].p, a[1].i, a[2].i, a[3].i, a[4].i, a[5].i, (int*)a[6].p,
+                              (float*)a[7].p, (int*)a[8].p, (int*)a[9].p, (int*)a[10].p, a[11].p,
+                              a[12].z, a[13].p);
+  return PyLong_FromLong(rc);
+}
+
+static PyObject* w_expert_combine(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  Arg a[11];
+  (void)self;
+  if (!p_expert_combine) return unbound("qkv_expert_combine"), NULL;
+  if (parse(args, n, "pipppp" "iiii" "p", a)) return NULL;
+  const int rc = p_expert_combine(a[0].p, a[1].i, (const int*)a[2].p, (const float*)a[3].p,
+                                  a[4].p, a[5].p, a[6].i, a[7].i, a[8].i, a[9].i, a[10].p);
+  return PyLong_FromLong(rc);
+}
+
 /* bind(name, address): point the wrapper of `name` at the loaded library's symbol */
 static PyObject* w_bind(PyObject* self, PyObject* args) {
   const char* name;
@@ -159,6 +207,11 @@ static PyObject* w_bind(PyObject* self, PyObject* args) {
   else if (!strcmp(name, "qkv_quantize_append_kv")) p_append_kv = (__typeof__(p_append_kv))f;
   else if (!strcmp(name, "qkv_combine")) p_combine = (__typeof__(p_combine))f;
   else if (!strcmp(name, "qkv_gather_combine")) p_gather_combine = (__typeof__(p_gather_combine))f;
+  else if (!strcmp(name, "qkv_quantized_matmul"))
+    p_quantized_matmul = (__typeof__(p_quantized_matmul))f;
+  else if (!strcmp(name, "qkv_grouped_matmul")) p_grouped_matmul = (__typeof__(p_grouped_matmul))f;
+  else if (!strcmp(name, "qkv_route_topk")) p_route_topk = (__typeof__(p_route_topk))f;
+  else if (!strcmp(name, "qkv_expert_combine")) p_expert_combine = (__typeof__(p_expert_combine))f;
   else return PyErr_Format(PyExc_KeyError, "no binding for %s", name);
   Py_RETURN_NONE;
 }
@@ -172,6 +225,13 @@ static PyMethodDef methods[] = {
     {"combine", (PyCFunction)(void (*)(void))w_combine, METH_FASTCALL, "qkv_combine"},
     {"gather_combine", (PyCFunction)(void (*)(void))w_gather_combine, METH_FASTCALL,
      "qkv_gather_combine"},
+    {"quantized_matmul", (PyCFunction)(void (*)(void))w_quantized_matmul, METH_FASTCALL,
+     "qkv_quantized_matmul"},
+    {"grouped_matmul", (PyCFunction)(void (*)(void))w_grouped_matmul, METH_FASTCALL,
+     "qkv_grouped_matmul"},
+    {"route_topk", (PyCFunction)(void (*)(void))w_route_topk, METH_FASTCALL, "qkv_route_topk"},
+    {"expert_combine", (PyCFunction)(void (*)(void))w_expert_combine, METH_FASTCALL,
+     "qkv_expert_combine"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_qkvext", NULL, -1, methods,

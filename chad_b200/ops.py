@@ -11,7 +11,7 @@ import ctypes
 import functools
 import math
 import os
-from typing import Optional, Sequence, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -384,3 +384,208 @@ def check_device() -> None:
         raise DeviceWaitError(
             f"a libqkv kernel gave up on a bounded wait (status {v}): outputs since the last "
             "check are not trustworthy; the workspace has been zeroed")
+
+
+# --------------------------------------------------------------------------------------
+# projections and experts with 4-bit weights
+# --------------------------------------------------------------------------------------
+
+_ACT = {None: _lib.QKV_ACT_NONE, "swiglu": _lib.QKV_ACT_SWIGLU}
+
+
+def _check_weights(x: torch.Tensor, w, s, b, bits: int, group_size: int, lead: int) -> int:
+    """Layouts of x (..., K) and the weight triple with `lead` leading dims -> dtype code."""
+    dt = _DT.get(x.dtype)
+    if dt is None or dt == _lib.QKV_F32:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if s.dtype != x.dtype or b.dtype != x.dtype:
+        raise TypeError("scales and biases must have x's dtype")
+    if w.element_size() != 4 or w.is_floating_point():
+        raise TypeError("packed weights must be 32-bit integers")
+    if not (w.is_contiguous() and s.is_contiguous() and b.is_contiguous()):
+        raise ValueError("the quantized weight tensors must be contiguous")
+    k = x.shape[-1]
+    ws = w.shape
+    if len(ws) != lead or ws[-1] * 32 != k * bits:
+        raise ValueError(f"packed weights {tuple(ws)} do not match x (..., {k}) at {bits} bits")
+    if s.shape != b.shape or s.shape[:-1] != ws[:-1] or s.shape[-1] * group_size != k:
+        raise ValueError(f"scales {tuple(s.shape)} / biases {tuple(b.shape)} do not match weights "
+                         f"{tuple(ws)} and group_size {group_size}")
+    return dt
+
+
+def _check_out(out: torch.Tensor, shape, like: torch.Tensor) -> None:
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(shape)} tensor of {like.dtype}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _matmul_workspace_size(device: int, m: int, e: int, n: int, k: int, dt: int, act: int) -> int:
+    # the kernel choice depends on the current device's SM count: memoized per device
+    return int(_lib.load().qkv_matmul_workspace_size(m, e, n, k, dt, act))
+
+
+def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int = 4,
+                     group_size: int = GROUP_SIZE, *, activation: Optional[str] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mx.quantized_matmul equivalent: x (..., K) times the transpose of affine 4-bit weights.
+
+    w_quant = (w int32 (N, K/8), scales (N, K/64), biases (N, K/64)) in the layout of
+    `quantize`, scales and biases in x's dtype (bf16 or fp16). Returns (..., N); with
+    activation="swiglu" the first N/2 rows of the weights are the gate and the others the up
+    projection, and silu(gate) * up (..., N/2) comes back. Sums in fp32, one rounding. x may
+    be a 2-D view with a row stride (a multiple of 8 elements).
+    """
+    w, s, b = w_quant
+    dev = _need_cuda(x, w, s, b)
+    dt = _check_weights(x, w, s, b, bits, group_size, 2)
+    act = _ACT.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    n, k = w.shape[0], x.shape[-1]
+    shape = x.shape
+    if len(shape) == 2 and x.stride(1) == 1:
+        m, ldx = shape[0], x.stride(0) if shape[0] > 1 else k
+    elif x.is_contiguous():
+        m, ldx = x.numel() // max(k, 1), k
+    else:
+        raise ValueError("x must be contiguous, or 2-D with contiguous rows")
+    out_shape = (*shape[:-1], n // 2 if act else n)
+    if out is None:
+        out = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    else:
+        _need_cuda(x, out)
+        _check_out(out, out_shape, x)
+    idx = dev.index
+    with _on(dev):
+        need = _matmul_workspace_size(idx, m, 1, n, k, dt, act)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(_lib.fn("qkv_quantized_matmul")(
+            x.data_ptr(), ldx, w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
+            bits, group_size, dt, act, _ptr(ws), need, _stream(dev)))
+    if CHECK_EACH_CALL:
+        with _on(dev):
+            check_device()
+    return out
+
+
+def grouped_quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor],
+                             offsets: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
+                             bits: int = 4, group_size: int = GROUP_SIZE,
+                             activation: Optional[str] = None,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One product per expert over rows sorted by expert (mx.gather_qmm equivalent).
+
+    w_quant = (w (E, N, K/8), scales (E, N, K/64), biases (E, N, K/64)); offsets int32 (E+1):
+    rows offsets[e] .. offsets[e+1] - 1 of the result belong to expert e. Row r of the result
+    comes from x[rows[r]] (rows int32 (R,)) or from x[r]. Returns (R, N), or (R, N/2) with
+    activation="swiglu"; rows outside [offsets[0], offsets[E]) are not written (of a result
+    allocated here they are undefined). An entry of rows outside x reads a row of zeros.
+    """
+    w, s, b = w_quant
+    dev = _need_cuda(x, w, s, b, offsets, rows)
+    dt = _check_weights(x, w, s, b, bits, group_size, 3)
+    act = _ACT.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be 2-D with contiguous rows")
+    e, n = w.shape[:2]
+    t, k = x.shape
+    if offsets.dtype != torch.int32 or (rows is not None and rows.dtype != torch.int32):
+        raise TypeError("offsets and rows must be int32")
+    if offsets.shape != (e + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"offsets must be a contiguous ({e + 1},) tensor")
+    if rows is not None and (rows.dim() != 1 or not rows.is_contiguous()):
+        raise ValueError("rows must be a contiguous 1-D tensor")
+    r = t if rows is None else rows.shape[0]
+    out_shape = (r, n // 2 if act else n)
+    if out is None:
+        out = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+    else:
+        _need_cuda(x, out)
+        _check_out(out, out_shape, x)
+    idx = dev.index
+    with _on(dev):
+        need = _matmul_workspace_size(idx, r, e, n, k, dt, act)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(_lib.fn("qkv_grouped_matmul")(
+            x.data_ptr(), x.stride(0) if t > 1 else k, t, _ptr(rows), offsets.data_ptr(),
+            w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), r, e, n, k, bits,
+            group_size, dt, act, _ptr(ws), need, _stream(dev)))
+    if CHECK_EACH_CALL:
+        with _on(dev):
+            check_device()
+    return out
+
+
+class Routing(NamedTuple):
+    """route_topk's result, int32 but for the fp32 weights."""
+
+    experts: torch.Tensor  # (T, k) chosen experts, largest logit first
+    weights: torch.Tensor  # (T, k) their softmax weights
+    rows: torch.Tensor     # (T*k,) token of each pair, sorted by expert and then token
+    slots: torch.Tensor    # (T, k) sorted position of each pair
+    offsets: torch.Tensor  # (E+1,) first sorted pair of each expert
+
+
+def route_topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routing:
+    """Route tokens to the k largest of E <= 512 logits (T, E), bf16, fp16 or fp32.
+
+    Ties go to the lowest expert; the weights are the softmax over all logits, or over the
+    chosen ones with `normalize`; an expert at -inf weighs 0, and a NaN logit counts as the
+    largest and makes its token's weights NaN.
+    """
+    dev = _need_cuda(logits)
+    if logits.dim() != 2 or not logits.is_contiguous():
+        raise ValueError("logits must be a contiguous (T, E) tensor")
+    dt = dtype_code(logits)
+    t, e = logits.shape
+    if not 0 < k <= min(e, 16):
+        raise ValueError(f"k must be in 1..min(E, 16) (got {k} of {e})")
+    pairs = t * k
+    ints = torch.empty(3 * pairs + e + 1, dtype=torch.int32, device=logits.device)
+    weights = torch.empty((t, k), dtype=torch.float32, device=logits.device)
+    experts, slots = ints[:pairs].view(t, k), ints[pairs:2 * pairs].view(t, k)
+    rows, offsets = ints[2 * pairs:3 * pairs], ints[3 * pairs:]
+    base = ints.data_ptr()
+    with _on(dev):
+        need = int(_lib.load().qkv_route_workspace_size(t, e)) if t > 64 else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(_lib.fn("qkv_route_topk")(
+            logits.data_ptr(), dt, t, e, k, 1 if normalize else 0, base, weights.data_ptr(),
+            base + 8 * pairs, base + 4 * pairs, base + 12 * pairs, _ptr(ws), need, _stream(dev)))
+    return Routing(experts, weights, rows, slots, offsets)
+
+
+def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
+                   residual: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Weighted sum of every token's expert rows: (residual[t] +) sum_j weights[t,j] *
+    y[slots[t,j]] for y (R, N), slots int32 and weights fp32 (T, k). Sums in fp32 in j's
+    order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual.
+    """
+    dev = _need_cuda(y, slots, weights, residual)
+    if y.dim() != 2 or slots.dim() != 2 or slots.shape != weights.shape:
+        raise ValueError("y must be (R, N), slots and weights (T, k)")
+    if slots.dtype != torch.int32 or weights.dtype != torch.float32:
+        raise TypeError("slots must be int32 and weights float32")
+    if not (y.is_contiguous() and slots.is_contiguous() and weights.is_contiguous()):
+        raise ValueError("y, slots and weights must be contiguous")
+    dt = dtype_code(y)
+    if dt == _lib.QKV_F32:
+        raise TypeError(f"unsupported dtype {y.dtype}")
+    r, n = y.shape
+    t, k = slots.shape
+    if residual is not None:
+        _check_out(residual, (t, n), y)
+    if out is None:
+        out = torch.empty((t, n), dtype=y.dtype, device=y.device)
+    else:
+        _need_cuda(y, out)
+        _check_out(out, (t, n), y)
+    with _on(dev):
+        check(_lib.fn("qkv_expert_combine")(
+            y.data_ptr(), r, slots.data_ptr(), weights.data_ptr(), _ptr(residual),
+            out.data_ptr(), t, k, n, dt, _stream(dev)))
+    return out

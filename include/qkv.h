@@ -57,6 +57,10 @@ extern "C" {
 #define QKV_OUT_NORMALIZED 0 /* out: (B,HQ,S,D) in the query dtype */
 #define QKV_OUT_PARTIAL 1    /* out: float (B,HQ,S,D+4) rows of [O(D), m, l, 0, 0] */
 
+/* activations of qkv_quantized_matmul / qkv_grouped_matmul */
+#define QKV_ACT_NONE 0
+#define QKV_ACT_SWIGLU 1 /* rows [0,N/2) of W are the gate, [N/2,N) the up projection */
+
 /* Library version (major*10000 + minor*100 + patch). */
 int qkv_version(void);
 
@@ -239,6 +243,69 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
                           int group_size, int dtype, float scale, int mask_kind,
                           const void* mask, int mask_nk, long long mask_sb, long long mask_sh,
                           long long mask_sq, int out_kind, int splits, void* stream);
+
+/*
+ * Products with affine 4-bit weights, the projections around the attention: the counterpart
+ * of mx.quantized_matmul (transpose=True), which the reference's models call with weights in
+ * the format of the cache (tests/test_engine_kvquant.py:22-37).
+ *
+ *   y = act(x W^T),  W[n][k] = scales[n][k/64] * code[n][k] + biases[n][k/64]
+ *
+ * x (M, K) with ldx elements between rows (a multiple of 8, at least K), w (N, K/8) uint32,
+ * scales and biases (N, K/64), out (M, N); x, scales, biases and out in `dtype` (bf16 or f16),
+ * sums in fp32, one rounding at the end. bits 4, group_size 64, K a multiple of 64. With
+ * QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
+ * x and w 16-byte aligned, the others naturally. Non-finite x makes its own row of out
+ * non-finite (inf or NaN) and no other. M = 0 does nothing.
+ * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter.
+ */
+size_t qkv_matmul_workspace_size(int M, int E, int N, int K, int dtype, int act);
+int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void* scales,
+                         const void* biases, void* out, int M, int N, int K, int bits,
+                         int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
+                         void* stream);
+
+/*
+ * The same with one weight matrix per expert over R rows sorted by expert (the counterpart of
+ * mx.gather_qmm in the reference's mixture-of-experts layers, src/chad/mlx_moe_fused.py):
+ *
+ *   out[r] = act(x[rows ? rows[r] : r] W_e^T)   for offsets[e] <= r < offsets[e+1]
+ *
+ * w (E, N, K/8), scales and biases (E, N, K/64), offsets device int32[E+1] (ascending, within
+ * [0, R]), rows device int32[R] or NULL. Rows of out outside [offsets[0], offsets[E]) are not
+ * written. Offsets outside [0, R] are clamped and a decreasing pair is an empty expert; an
+ * entry of rows outside [0, x_rows) reads a row of zeros.
+ */
+int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows,
+                       const int* offsets, const void* w, const void* scales,
+                       const void* biases, void* out, int R, int E, int N, int K, int bits,
+                       int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
+                       void* stream);
+
+/*
+ * Route T tokens to k of E experts (E <= 512, k <= 16, k <= E): logits (T, E) in `dtype`
+ * (bf16, f16 or f32). experts, weights (T, k): the k largest logits in descending order (ties
+ * to the lowest expert; a NaN counts as the largest and makes its token's weights NaN) and
+ * their softmax over all E logits, or over the chosen k with normalize != 0; an expert whose
+ * logit is -inf weighs 0. The pairs sorted by expert, then token: offsets (E+1), rows (T*k)
+ * the token of each sorted pair, slots (T, k) the sorted position of each pair. Integers are
+ * int32. workspace: qkv_route_workspace_size bytes (0: may be NULL), contents don't matter.
+ * (The top-k softmax gate in front of the reference's fused expert kernels,
+ * src/chad/mlx_moe_fused.py.)
+ */
+size_t qkv_route_workspace_size(int T, int E);
+int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int normalize,
+                   int* experts, float* weights, int* rows, int* slots, int* offsets,
+                   void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]]: the experts' rows y (R, N) back
+ * in token order, in fp32 and j's order, rounded once. slots (T, k) int32, weights (T, k) fp32,
+ * residual (T, N) or NULL, out (T, N) (may be the residual); a slot outside [0, R) adds nothing.
+ */
+int qkv_expert_combine(const void* y, int R, const int* slots, const float* weights,
+                       const void* residual, void* out, int T, int k, int N, int dtype,
+                       void* stream);
 
 #ifdef __cplusplus
 }
