@@ -28,6 +28,9 @@ struct MatmulArgs {
 };
 
 int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st);  // few rows per weight matrix
+int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st);    // many (tcgen05)
+bool matmul_tc_fits(int E, int N);  // whether the tcgen05 kernel takes the stacked weights
+int launch_matmul(const MatmulArgs& a, cudaStream_t st);       // whichever is faster
 
 struct RouteArgs {
   const void* logits;  // (T, E) in dtype

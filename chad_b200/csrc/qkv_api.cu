@@ -507,7 +507,7 @@ int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void
   int rc = setup_matmul(a, x, ldx, M, nullptr, nullptr, w, scales, biases, out, M, 1, N, K, bits,
                         group_size, dtype, act, workspace, ws_bytes);
   if (rc || M == 0) return rc;
-  rc = launch_matmul_rows(a, static_cast<cudaStream_t>(stream));
+  rc = launch_matmul(a, static_cast<cudaStream_t>(stream));
   if (rc) return fail(rc, "quantized_matmul: unsupported shape");
   return cuda_check("qkv_quantized_matmul");
 }
@@ -518,12 +518,13 @@ int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows
                        int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
                        void* stream) {
   if (R > 0 && !offsets) return fail(QKV_EINVAL, "null offsets");
+  if (rows && R > 0 && x_rows == 0) return fail(QKV_EINVAL, "rows of an x that has none");
   if (!rows && R > x_rows) return fail(QKV_EINVAL, "R %d exceeds the %d rows of x", R, x_rows);
   MatmulArgs a;
   int rc = setup_matmul(a, x, ldx, x_rows, rows, offsets, w, scales, biases, out, R, E, N, K,
                         bits, group_size, dtype, act, workspace, ws_bytes);
   if (rc || R == 0) return rc;
-  rc = launch_matmul_rows(a, static_cast<cudaStream_t>(stream));
+  rc = launch_matmul(a, static_cast<cudaStream_t>(stream));
   if (rc) return fail(rc, "grouped_matmul: unsupported shape");
   return cuda_check("qkv_grouped_matmul");
 }

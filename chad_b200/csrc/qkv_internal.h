@@ -122,6 +122,11 @@ bool make_code_map_bytes(CUtensorMap* m, const void* base, int RB, int NP, long 
                          int box_inner, int box_rows);
 
 
+// Tiled tensor map over `rows` rows of `inner` elements (1 or 2 bytes), box (box_inner,
+// box_rows) with box_inner spanning 128 bytes, 128-byte swizzle.
+bool make_rows_map(CUtensorMap* m, const void* base, int elem_bytes, long long inner,
+                   long long rows, long long row_bytes, int box_inner, int box_rows);
+
 bool prefill_tc_eligible(int B, int HQ, int HKV, int S, int D, const int* lens,
                          const int* pos_base, const int* total_lens, int mask_kind);
 TcPlan prefill_tc_plan(int B, int HQ, int HKV, int S, int n_max, int want_splits);

@@ -70,6 +70,8 @@ MATMUL = [
     (9, 64, 512), (13, 255, 1088), (16, 129, 2048), (17, 40, 576), (31, 257, 704), (64, 300, 1024),
     (65, 128, 256), (130, 200, 320), (257, 96, 832), (300, 513, 64), (1, 5000, 2048),
     (1, 40000, 128), (5, 20001, 320), (40, 9000, 192),
+    # more K than any ring of shared-memory stages holds, twice over
+    (3, 1000, 4096), (33, 600, 6144), (200, 1300, 4096), (192, 130, 6208),
 ]
 
 
