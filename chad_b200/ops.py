@@ -391,27 +391,28 @@ def check_device() -> None:
 # --------------------------------------------------------------------------------------
 
 _ACT = {None: _lib.QKV_ACT_NONE, "swiglu": _lib.QKV_ACT_SWIGLU}
+_DT16 = {torch.bfloat16: _lib.QKV_BF16, torch.float16: _lib.QKV_F16}
+_INT32 = (torch.int32, torch.uint32)
 
 
-def _check_weights(x: torch.Tensor, w, s, b, bits: int, group_size: int, lead: int) -> int:
-    """Layouts of x (..., K) and the weight triple with `lead` leading dims -> dtype code."""
-    dt = _DT.get(x.dtype)
-    if dt is None or dt == _lib.QKV_F32:
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _refuse_weights(x: torch.Tensor, w, s, b, bits: int, group_size: int, lead: int):
+    """Raise for what the callers' one-line test of x (..., K) and the weight triple (with
+    `lead` leading dimensions) found wrong."""
+    if x.dtype not in _DT16:
         raise TypeError(f"unsupported dtype {x.dtype}")
     if s.dtype != x.dtype or b.dtype != x.dtype:
         raise TypeError("scales and biases must have x's dtype")
-    if w.element_size() != 4 or w.is_floating_point():
+    if w.dtype not in _INT32:
         raise TypeError("packed weights must be 32-bit integers")
     if not (w.is_contiguous() and s.is_contiguous() and b.is_contiguous()):
         raise ValueError("the quantized weight tensors must be contiguous")
-    k = x.shape[-1]
-    ws = w.shape
-    if len(ws) != lead or ws[-1] * 32 != k * bits:
-        raise ValueError(f"packed weights {tuple(ws)} do not match x (..., {k}) at {bits} bits")
-    if s.shape != b.shape or s.shape[:-1] != ws[:-1] or s.shape[-1] * group_size != k:
-        raise ValueError(f"scales {tuple(s.shape)} / biases {tuple(b.shape)} do not match weights "
-                         f"{tuple(ws)} and group_size {group_size}")
-    return dt
+    raise ValueError(f"packed weights {tuple(w.shape)}, scales {tuple(s.shape)} and biases "
+                     f"{tuple(b.shape)} do not match x (..., {x.shape[-1] if x.dim() else ''}) at "
+                     f"{bits} bits, {lead} leading dimensions and group_size {group_size}")
 
 
 def _check_out(out: torch.Tensor, shape, like: torch.Tensor) -> None:
@@ -436,36 +437,46 @@ def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int
     projection, and silu(gate) * up (..., N/2) comes back. Sums in fp32, one rounding. x may
     be a 2-D view with a row stride (a multiple of 8 elements).
     """
+    # one call per projection per decode step: the host work is kept to plain attribute reads
     w, s, b = w_quant
-    dev = _need_cuda(x, w, s, b)
-    dt = _check_weights(x, w, s, b, bits, group_size, 2)
+    idx = x.get_device()
+    if idx < 0 or w.get_device() != idx or s.get_device() != idx or b.get_device() != idx:
+        _need_cuda(x, w, s, b)
+    shape, ws, tp = x.shape, w.shape, x.dtype
+    dt = _DT16.get(tp)
+    k = shape[-1] if shape else 0
+    n = ws[0] if ws else 0
+    if (dt is None or s.dtype is not tp or b.dtype is not tp or w.dtype not in _INT32
+            or ws != (n, k * bits // 32) or s.shape != (n, k // group_size)
+            or b.shape != s.shape or not w.is_contiguous() or not s.is_contiguous()
+            or not b.is_contiguous()):
+        _refuse_weights(x, w, s, b, bits, group_size, 1)
     act = _ACT.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    n, k = w.shape[0], x.shape[-1]
-    shape = x.shape
-    if len(shape) == 2 and x.stride(1) == 1:
-        m, ldx = shape[0], x.stride(0) if shape[0] > 1 else k
-    elif x.is_contiguous():
+    if x.is_contiguous():
         m, ldx = x.numel() // max(k, 1), k
+    elif len(shape) == 2 and x.stride(1) == 1:
+        m, ldx = shape[0], x.stride(0)
     else:
         raise ValueError("x must be contiguous, or 2-D with contiguous rows")
     out_shape = (*shape[:-1], n // 2 if act else n)
     if out is None:
-        out = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(out_shape)
     else:
         _need_cuda(x, out)
         _check_out(out, out_shape, x)
-    idx = dev.index
-    with _on(dev):
-        need = _matmul_workspace_size(idx, m, 1, n, k, dt, act)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(_lib.fn("qkv_quantized_matmul")(
-            x.data_ptr(), ldx, w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
-            bits, group_size, dt, act, _ptr(ws), need, _stream(dev)))
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return quantized_matmul(x, w_quant, bits, group_size, activation=activation, out=out)
+    need = _matmul_workspace_size(idx, m, 1, n, k, dt, act)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(_lib.fn("qkv_quantized_matmul")(
+        x.data_ptr(), ldx, w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
+        bits, group_size, dt, act, _ptr(work), need,
+        _RAW_STREAM(idx) if _RAW_STREAM is not None else _stream(x.device)))
     if CHECK_EACH_CALL:
-        with _on(dev):
-            check_device()
+        check_device()
     return out
 
 
@@ -483,16 +494,25 @@ def grouped_quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor],
     allocated here they are undefined). An entry of rows outside x reads a row of zeros.
     """
     w, s, b = w_quant
-    dev = _need_cuda(x, w, s, b, offsets, rows)
-    dt = _check_weights(x, w, s, b, bits, group_size, 3)
+    idx = x.get_device()
+    if (idx < 0 or w.get_device() != idx or s.get_device() != idx or b.get_device() != idx
+            or offsets.get_device() != idx or (rows is not None and rows.get_device() != idx)):
+        _need_cuda(x, w, s, b, offsets, rows)
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be 2-D with contiguous rows")
+    t, k = x.shape
+    ws, tp = w.shape, x.dtype
+    dt = _DT16.get(tp)
+    e, n = (ws[0], ws[1]) if len(ws) == 3 else (0, 0)
+    if (dt is None or s.dtype is not tp or b.dtype is not tp or w.dtype not in _INT32
+            or ws != (e, n, k * bits // 32) or s.shape != (e, n, k // group_size)
+            or b.shape != s.shape or not w.is_contiguous() or not s.is_contiguous()
+            or not b.is_contiguous()):
+        _refuse_weights(x, w, s, b, bits, group_size, 2)
     act = _ACT.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError("x must be 2-D with contiguous rows")
-    e, n = w.shape[:2]
-    t, k = x.shape
-    if offsets.dtype != torch.int32 or (rows is not None and rows.dtype != torch.int32):
+    if offsets.dtype is not torch.int32 or (rows is not None and rows.dtype is not torch.int32):
         raise TypeError("offsets and rows must be int32")
     if offsets.shape != (e + 1,) or not offsets.is_contiguous():
         raise ValueError(f"offsets must be a contiguous ({e + 1},) tensor")
@@ -501,21 +521,23 @@ def grouped_quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor],
     r = t if rows is None else rows.shape[0]
     out_shape = (r, n // 2 if act else n)
     if out is None:
-        out = torch.empty(out_shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(out_shape)
     else:
         _need_cuda(x, out)
         _check_out(out, out_shape, x)
-    idx = dev.index
-    with _on(dev):
-        need = _matmul_workspace_size(idx, r, e, n, k, dt, act)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(_lib.fn("qkv_grouped_matmul")(
-            x.data_ptr(), x.stride(0) if t > 1 else k, t, _ptr(rows), offsets.data_ptr(),
-            w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), r, e, n, k, bits,
-            group_size, dt, act, _ptr(ws), need, _stream(dev)))
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return grouped_quantized_matmul(x, w_quant, offsets, rows=rows, bits=bits,
+                                            group_size=group_size, activation=activation, out=out)
+    need = _matmul_workspace_size(idx, r, e, n, k, dt, act)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(_lib.fn("qkv_grouped_matmul")(
+        x.data_ptr(), x.stride(0) if t > 1 else k, t, _ptr(rows), offsets.data_ptr(),
+        w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), r, e, n, k, bits,
+        group_size, dt, act, _ptr(work), need,
+        _RAW_STREAM(idx) if _RAW_STREAM is not None else _stream(x.device)))
     if CHECK_EACH_CALL:
-        with _on(dev):
-            check_device()
+        check_device()
     return out
 
 
@@ -536,26 +558,36 @@ def route_topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routi
     chosen ones with `normalize`; an expert at -inf weighs 0, and a NaN logit counts as the
     largest and makes its token's weights NaN.
     """
-    dev = _need_cuda(logits)
+    idx = logits.get_device()
+    if idx < 0:
+        _need_cuda(logits)
     if logits.dim() != 2 or not logits.is_contiguous():
         raise ValueError("logits must be a contiguous (T, E) tensor")
     dt = dtype_code(logits)
     t, e = logits.shape
     if not 0 < k <= min(e, 16):
         raise ValueError(f"k must be in 1..min(E, 16) (got {k} of {e})")
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return route_topk(logits, k, normalize=normalize)
     pairs = t * k
-    ints = torch.empty(3 * pairs + e + 1, dtype=torch.int32, device=logits.device)
-    weights = torch.empty((t, k), dtype=torch.float32, device=logits.device)
-    experts, slots = ints[:pairs].view(t, k), ints[pairs:2 * pairs].view(t, k)
-    rows, offsets = ints[2 * pairs:3 * pairs], ints[3 * pairs:]
+    need = _route_workspace_size(t, e)
+    # one allocation for the integers: offsets, rows, experts, slots and the workspace
+    ints = logits.new_empty(e + 1 + 3 * pairs + need // 4 + 4, dtype=torch.int32)
+    weights = logits.new_empty((t, k), dtype=torch.float32)
+    offsets, rows, experts, slots, work = ints.split((e + 1, pairs, pairs, pairs, need // 4 + 4))
     base = ints.data_ptr()
-    with _on(dev):
-        need = int(_lib.load().qkv_route_workspace_size(t, e)) if t > 64 else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(_lib.fn("qkv_route_topk")(
-            logits.data_ptr(), dt, t, e, k, 1 if normalize else 0, base, weights.data_ptr(),
-            base + 8 * pairs, base + 4 * pairs, base + 12 * pairs, _ptr(ws), need, _stream(dev)))
-    return Routing(experts, weights, rows, slots, offsets)
+    at = base + 4 * (e + 1)
+    check(_lib.fn("qkv_route_topk")(
+        logits.data_ptr(), dt, t, e, k, 1 if normalize else 0, at + 4 * pairs,
+        weights.data_ptr(), at, at + 8 * pairs, base, (at + 12 * pairs + 15) & ~15, need,
+        _RAW_STREAM(idx) if _RAW_STREAM is not None else _stream(logits.device)))
+    return Routing(experts.view(t, k), weights, rows, slots.view(t, k), offsets)
+
+
+@functools.lru_cache(maxsize=4096)
+def _route_workspace_size(t: int, e: int) -> int:
+    return int(_lib.load().qkv_route_workspace_size(t, e))
 
 
 def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, *,
@@ -565,27 +597,33 @@ def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, 
     y[slots[t,j]] for y (R, N), slots int32 and weights fp32 (T, k). Sums in fp32 in j's
     order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual.
     """
-    dev = _need_cuda(y, slots, weights, residual)
-    if y.dim() != 2 or slots.dim() != 2 or slots.shape != weights.shape:
+    idx = y.get_device()
+    if (idx < 0 or slots.get_device() != idx or weights.get_device() != idx
+            or (residual is not None and residual.get_device() != idx)):
+        _need_cuda(y, slots, weights, residual)
+    shape = slots.shape
+    if y.dim() != 2 or len(shape) != 2 or shape != weights.shape:
         raise ValueError("y must be (R, N), slots and weights (T, k)")
-    if slots.dtype != torch.int32 or weights.dtype != torch.float32:
+    if slots.dtype is not torch.int32 or weights.dtype is not torch.float32:
         raise TypeError("slots must be int32 and weights float32")
     if not (y.is_contiguous() and slots.is_contiguous() and weights.is_contiguous()):
         raise ValueError("y, slots and weights must be contiguous")
-    dt = dtype_code(y)
-    if dt == _lib.QKV_F32:
+    dt = _DT16.get(y.dtype)
+    if dt is None:
         raise TypeError(f"unsupported dtype {y.dtype}")
     r, n = y.shape
-    t, k = slots.shape
+    t, k = shape
     if residual is not None:
         _check_out(residual, (t, n), y)
     if out is None:
-        out = torch.empty((t, n), dtype=y.dtype, device=y.device)
+        out = y.new_empty((t, n))
     else:
         _need_cuda(y, out)
         _check_out(out, (t, n), y)
-    with _on(dev):
-        check(_lib.fn("qkv_expert_combine")(
-            y.data_ptr(), r, slots.data_ptr(), weights.data_ptr(), _ptr(residual),
-            out.data_ptr(), t, k, n, dt, _stream(dev)))
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return expert_combine(y, slots, weights, residual=residual, out=out)
+    check(_lib.fn("qkv_expert_combine")(
+        y.data_ptr(), r, slots.data_ptr(), weights.data_ptr(), _ptr(residual), out.data_ptr(), t,
+        k, n, dt, _RAW_STREAM(idx) if _RAW_STREAM is not None else _stream(y.device)))
     return out
