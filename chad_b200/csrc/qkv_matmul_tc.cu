@@ -12,8 +12,9 @@
 //     an expert's rows are cut into equal tiles. Every CTA takes a contiguous range of the
 //     tiles of equal summed cost, computed by each CTA from the offsets: nothing is counted
 //     through memory, and neighbouring tiles share rows of x in L2.
-//   * Warps: 0-7 dequantize (two warpgroups, even and odd K steps), 8-11 store results,
-//     12-15 load rows of x, 16 issues the MMAs.
+//   * Warps: 0 issues the MMAs, 1 loads rows of x (TMA), 2 packed codes (TMA), 4-11
+//     dequantize (two warpgroups, alternate 128 K values), 12-15 store results; 1, 3 and 16-19
+//     gather rows of x (TMA, four rows a load).
 //   * Tensor memory: two accumulators of 192 columns (a tile's results are stored while the
 //     next one accumulates) and four A stages of 32 columns (64 K values each).
 //   * Gated activation: 16 gate rows and the 16 up rows of the same outputs share a warp's 32
@@ -37,7 +38,7 @@ namespace qkv {
 
 namespace {
 
-constexpr int kWarps = 18;
+constexpr int kWarps = 20;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxTok = 192;           // rows of x in a tile
 constexpr int kAStages = 2;            // of 128 K values, in tensor memory
@@ -47,6 +48,10 @@ constexpr int kMaxBStages = 8;         // of 128 K values
 constexpr int kBBytes = 144 * 1024;    // shared memory of the B stages
 constexpr int kSlots = 4;              // prefetched spans of packed codes
 constexpr int kSlotBytes = 128 * 128;  // 128 weight rows x 128 bytes: 256 K values
+// barriers, in shared memory: pairs of full and free by stage
+constexpr int kBarA = 0, kBarB = kBarA + 2 * kAStages, kBarC = kBarB + 2 * kMaxBStages;
+constexpr int kBarAcc = kBarC + 2 * kSlots, kBarFin = kBarAcc + 4, kBars = kBarFin + 1;
+constexpr int kGatherWarps = 6;        // warps 1, 3 and 16-19
 constexpr int kMaxExperts = 1024;
 
 struct TcArgs {
@@ -110,11 +115,11 @@ struct Conv<__half> {
 
 // tile of `map` at (column, row) into shared memory
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int col, int row,
-                                          uint64_t* bar) {
+                                          uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
       "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(smem_u32(bar))
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(bar)
       : "memory");
 }
 // Scale loads, volatile so that they stay ahead of the span they are loaded under.
@@ -137,14 +142,15 @@ __device__ __forceinline__ bool bad_row(const MatmulArgs& a, int r) {
   const int i = __ldg(a.rows + r);
   return i < 0 || i >= a.x_rows;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// four rows of `map` (any indices inside it) at a column
+__device__ __forceinline__ void load_rows4(uint32_t dst, const CUtensorMap* map, int col,
+                                           const int4& r, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w),
+      "r"(bar)
+      : "memory");
 }
 // one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
@@ -154,11 +160,74 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// mbar_wait whose first polls skip the timer: K steps are a fraction of a microsecond apart.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status, int where) {
-  for (int i = 0; i < 64; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, status, where);
+// Barrier waits by shared address: one poll inline; a wait that lasts suspends in hardware
+// until the phase flips (polling would take issue slots from the dequantizers), bounded as
+// every wait of the library.
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status, int where) {
+  unsigned long long t0 = 0;
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(100000u)
+        : "memory");
+    if (ok) return true;
+    if (i >= 4) {
+      const unsigned long long t = global_ns();
+      if (!t0) t0 = t;
+      if (t - t0 > kSpinNanos) break;
+    }
+  }
+  flag_device_error(status, where);
+  return false;
+}
+// one thread
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int* status, int where) {
+  return poll(bar, parity) || wait_long(bar, parity, status, where);
+}
+// a converged warp, which stays converged
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status, int where) {
+  if (__all_sync(0xffffffffu, poll(bar, parity))) return true;
+  return __all_sync(0xffffffffu, wait_long(bar, parity, status, where));
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(
+          bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+// four MMAs of 16 K values: A from tensor memory, B's descriptor by halves
+__device__ __forceinline__ void mma4(uint32_t acc, uint32_t at, uint32_t blo, uint32_t bhi,
+                                     uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 d;\n\tmov.b64 d, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, p;\n\t}" ::"r"(acc),
+        "r"(at + s * 8), "r"(blo + s * 2), "r"(bhi), "r"(idesc), "r"(s ? 1u : accumulate)
+        : "memory");
 }
 
 // Walks this CTA's tiles: expert, row tile, weight tile (fastest).
@@ -199,9 +268,7 @@ struct Cursor {
 template <typename T, bool GATED, int SB>
 __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_constant__ TcArgs p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ uint64_t a_full[kAStages], a_free[kAStages], b_full[kMaxBStages], b_free[kMaxBStages];
-  __shared__ uint64_t c_full[kSlots], c_free[kSlots];
-  __shared__ uint64_t acc_full[2], acc_free[2], mma_fin;
+  __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_sh;
   __shared__ int start_sh[3];
   __shared__ long long range_sh[2];
@@ -215,32 +282,32 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   // ---- set-up: barriers, tensor memory, this CTA's range of tiles --------------------------
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAStages; ++i) {
-      mbar_init(&a_full[i], 4);
-      mbar_init(&a_free[i], 1);
+      mbar_init(&bars[kBarA + 2 * i], 4);
+      mbar_init(&bars[kBarA + 2 * i + 1], 1);
     }
     for (int i = 0; i < kMaxBStages; ++i) {
-      mbar_init(&b_full[i], a.rows ? 4 : 1);
-      mbar_init(&b_free[i], 1);
+      mbar_init(&bars[kBarB + 2 * i], a.rows ? kGatherWarps : 1);
+      mbar_init(&bars[kBarB + 2 * i + 1], 1);
     }
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&c_full[i], 1);
-      mbar_init(&c_free[i], 8);
+      mbar_init(&bars[kBarC + 2 * i], 1);
+      mbar_init(&bars[kBarC + 2 * i + 1], 8);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_free[i], 4);
+      mbar_init(&bars[kBarAcc + 2 * i], 1);
+      mbar_init(&bars[kBarAcc + 2 * i + 1], 4);
     }
-    mbar_init(&mma_fin, 1);
+    mbar_init(&bars[kBarFin], 1);
     fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == 0) {
     tc::tmem_alloc(&tmem_sh, 512);
     tc::tmem_relinquish();
   }
   for (int e = threadIdx.x; e <= a.E; e += kThreads)
     off[e] = a.offsets ? min(max(a.offsets[e], 0), a.R) : (e ? a.R : 0);
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 3) {
     // total cost, then the first tile that starts inside this CTA's share
     long long total = 0;
     for (int e = lane; e < a.E; e += 32) {
@@ -303,11 +370,14 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   if (cur.e < a.E) cur.set_expert();
   const int n_out = GATED ? a.N / 2 : a.N;
   const int half_bytes = p.tok * 128;  // a B stage is two tiles of 64 K values
+  // full barrier of A stage i at bar_a + 16 i, its free barrier 8 bytes on; the others alike
+  const uint32_t bar_a = smem_u32(bars), bar_b = bar_a + 8 * kBarB, bar_c = bar_a + 8 * kBarC;
+  const uint32_t bar_acc = bar_a + 8 * kBarAcc, bar_fin = bar_a + 8 * kBarFin;
   bool ok = true;
 
-  if (warp < 8) {
+  if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------------ dequantizers
-    const int par = warp >> 2, q = warp & 3;  // double step of a span; tensor memory lanes 32q..32q+31
+    const int par = (warp >> 2) - 1, q = warp & 3;  // double step of a span; tensor memory lanes 32q..32q+31
     const int spans = (steps + 3) / 4;
     const uint32_t my_row = smem_u32(codes) + (q * 32 + lane) * 128;
     int slot = 0;
@@ -372,15 +442,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           }
           if (span + 1 < spans) load_sb(span + 1);
         }
-        ok = __all_sync(0xffffffffu, wait(&c_full[slot], ph, a.status, 67));
+        ok = wait_warp(bar_c + 16 * slot, ph, a.status, 67);
         if (!ok) break;
         const int k0 = span * 4 + 2 * par;  // this warpgroup's steps k0 and k0 + 1
         if (k0 < steps) {
           const uint32_t g = gs + span * 2 + par, st = g % kAStages;
-          ok = __all_sync(0xffffffffu,
-                          wait(&a_free[st], ((g / kAStages) & 1) ^ 1, a.status, 60));
-          if (!ok) break;
-          tc::fence_after_sync();
+          const uint32_t dst = tmem + kACol + st * kACols + ((uint32_t)(q * 32) << 16);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t out[32];
@@ -408,18 +475,25 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
                 out[16 * i + 4 * w + 3] = prmt(v[2], v[3], 0x7632);
               }
             }
+            // the first half is converted before the stage is free
+            if (h == 0) {
+              ok = wait_warp(bar_a + 16 * st + 8, ((g / kAStages) & 1) ^ 1, a.status, 60);
+              if (!ok) break;
+              tc::fence_after_sync();
+            }
             // (the second half of an odd last step holds zeros that no MMA reads)
-            tc::st32(tmem + kACol + st * kACols + h * 32 + ((uint32_t)(q * 32) << 16), out);
+            tc::st32(dst + h * 32, out);
           }
+          if (!ok) break;
           tc::wait_st();
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&a_full[st]);
+          if (lane == 0) arrive(bar_a + 16 * st);
         }
         // after the last use of the words, not after their loads: a load that the assembler
         // moved below this arrive would read the slot's next contents
         __syncwarp();
-        if (lane == 0) mbar_arrive(&c_free[slot]);
+        if (lane == 0) arrive(bar_c + 16 * slot + 8);
         if (++slot == kSlots) {
           slot = 0;
           ph ^= 1;
@@ -428,14 +502,14 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       gs += (steps + 1) / 2;
       cur.next();
     }
-  } else if (warp < 12) {
+  } else if (warp >= 12 && warp < 16) {
     // ------------------------------------------------------------------ results
     const int q = warp & 3;
     int tile = 0;
     T* out = (T*)a.out;
     while (cur.valid()) {
       const int buf = tile & 1;
-      ok = __all_sync(0xffffffffu, wait(&acc_full[buf], (tile >> 1) & 1, a.status, 61));
+      ok = wait_warp(bar_acc + 16 * buf, (tile >> 1) & 1, a.status, 61);
       if (!ok) break;
       tc::fence_after_sync();
       const int row0 = cur.row0(), rows = cur.row1() - row0;
@@ -480,62 +554,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       }
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_free[buf]);
+      if (lane == 0) arrive(bar_acc + 16 * buf + 8);
       ++tile;
       cur.next();
     }
-  } else if (warp < 16 && a.rows) {
-    // ------------------------------------------------------------------ gathered rows of x
-    const int tid = threadIdx.x - 12 * 32;
-    const int c = tid & 7, r0 = tid >> 3;  // 16-byte chunk of 64 K values; rows r0 + 16 i
-    const uint32_t base = smem_u32(smem) + r0 * 128 + ((c ^ (r0 & 7)) << 4);
-    int st = 0, done_st = 0;
-    uint32_t ph = 1;
-    bool pending = false;  // the stage before is still landing
-    auto landed = [&]() {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b_full[done_st]);
-      done_st = done_st + 1 == p.b_stages ? 0 : done_st + 1;
-    };
-    while (cur.valid() && ok) {
-      const int row0 = cur.row0(), row1 = cur.row1();
-      const int n16 = (row1 - row0 + 15) / 16;
-      const char* src[kMaxTok / 16];
-#pragma unroll
-      for (int i = 0; i < kMaxTok / 16; ++i) {
-        const int r = row0 + r0 + 16 * i;
-        int from = r < row1 ? __ldg(a.rows + r) : 0;
-        if (from < 0 || from >= a.x_rows) from = 0;  // (the results of these rows are zeroed)
-        src[i] = (const char*)a.x + ((long long)from * a.ldx + c * 8) * 2;
-      }
-      for (int k = 0; k < steps; k += 2) {
-        ok = __all_sync(0xffffffffu, wait(&b_free[st], ph, a.status, 62));
-        if (!ok) break;
-        const uint32_t dst = base + st * 2 * half_bytes;
-#pragma unroll
-        for (int i = 0; i < kMaxTok / 16; ++i)
-          if (i < n16) {
-            cp16(dst + i * 2048, src[i] + (long long)k * 128, 16);
-            if (k + 1 < steps) cp16(dst + half_bytes + i * 2048, src[i] + (long long)k * 128 + 128, 16);
-          }
-        cp_commit();
-        if (++st == p.b_stages) {
-          st = 0;
-          ph ^= 1;
-        }
-        if (pending) {
-          cp_wait<1>();
-          landed();
-        }
-        pending = true;
-      }
-      cur.next();
-    }
-    cp_wait<0>();
-    if (pending) landed();
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ rows of x in order
+  } else if (warp == 1 && !a.rows) {
+    // ------------------------------------------------------------------ rows of x, in order
     if (lane == 0) {
       const uint32_t base = smem_u32(smem);
       int st = 0, issued = 0;
@@ -543,12 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       while (cur.valid() && ok) {
         const int row0 = cur.row0();
         for (int k = 0; k < steps; k += 2) {
-          ok = wait(&b_free[st], ph, a.status, 62);
+          ok = wait_one(bar_b + 16 * st + 8, ph, a.status, 62);
           if (!ok) break;
           const uint32_t dst = base + st * 2 * half_bytes;
-          mbar_arrive_expect_tx(&b_full[st], k + 1 < steps ? 2 * half_bytes : half_bytes);
-          load_tile(dst, &p.x, k * 64, row0, &b_full[st]);
-          if (k + 1 < steps) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, &b_full[st]);
+          arrive_tx(bar_b + 16 * st, k + 1 < steps ? 2 * half_bytes : half_bytes);
+          load_tile(dst, &p.x, k * 64, row0, bar_b + 16 * st);
+          if (k + 1 < steps) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar_b + 16 * st);
           ++issued;
           if (++st == p.b_stages) {
             st = 0;
@@ -561,10 +585,56 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       for (int i = min(issued, p.b_stages); i > 0; --i) {
         st = st ? st - 1 : p.b_stages - 1;
         if (st == p.b_stages - 1) ph ^= 1;
-        wait(&b_full[st], ph ^ 1, a.status, 68);
+        wait_one(bar_b + 16 * st, ph ^ 1, a.status, 68);
       }
     }
-  } else if (warp == 17) {
+  } else if (a.rows && (warp == 1 || warp == 3 || warp >= 16)) {
+    // ------------------------------------------------------------------ rows of x, gathered
+    // four rows per load; a load instruction takes a thread about 44 clocks, so six warps
+    const uint32_t base = smem_u32(smem);
+    const int w = warp < 16 ? warp >> 1 : warp - 14;
+    int st = 0, issued = 0;
+    uint32_t ph = 1;
+    while (cur.valid() && ok) {
+      const int row0 = cur.row0(), row1 = cur.row1();
+      const int n4 = (row1 - row0 + 15) / 16 * 4;
+      const int four = w + kGatherWarps * lane;
+      const int mine = (n4 - w + kGatherWarps - 1) / kGatherWarps;  // fours of this warp
+      int4 idx = make_int4(0, 0, 0, 0);  // (bad and missing rows load row 0)
+      if (four < n4) {
+        int v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int r = row0 + four * 4 + c;
+          v[c] = r < row1 ? a.rows[r] : 0;
+          if (v[c] < 0 || v[c] >= a.x_rows) v[c] = 0;
+        }
+        idx = make_int4(v[0], v[1], v[2], v[3]);
+      }
+      for (int k = 0; k < steps; k += 2) {
+        ok = wait_warp(bar_b + 16 * st + 8, ph, a.status, 62);
+        if (!ok) break;
+        const uint32_t dst = base + st * 2 * half_bytes + four * 512;
+        if (lane == 0) arrive_tx(bar_b + 16 * st, mine * (k + 1 < steps ? 1024 : 512));
+        __syncwarp();
+        if (four < n4) {
+          load_rows4(dst, &p.x, k * 64, idx, bar_b + 16 * st);
+          if (k + 1 < steps) load_rows4(dst + half_bytes, &p.x, k * 64 + 64, idx, bar_b + 16 * st);
+        }
+        ++issued;
+        if (++st == p.b_stages) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+      cur.next();
+    }
+    for (int i = min(issued, p.b_stages); i > 0; --i) {
+      st = st ? st - 1 : p.b_stages - 1;
+      if (st == p.b_stages - 1) ph ^= 1;
+      wait_warp(bar_b + 16 * st, ph ^ 1, a.status, 68);
+    }
+  } else if (warp == 2) {
     // ------------------------------------------------------------------ packed codes
     if (lane == 0) {
       const uint32_t base = smem_u32(codes);
@@ -574,17 +644,17 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       while (cur.valid() && ok) {
         const int row = cur.e * a.N + cur.j * (GATED ? 64 : 128);
         for (int span = 0; span < spans; ++span) {
-          ok = wait(&c_free[slot], ph, a.status, 69);
+          ok = wait_one(bar_c + 16 * slot + 8, ph, a.status, 69);
           if (!ok) break;
           const uint32_t dst = base + slot * kSlotBytes;
-          mbar_arrive_expect_tx(&c_full[slot], kSlotBytes);
+          arrive_tx(bar_c + 16 * slot, kSlotBytes);
           if (GATED) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)  // 16 gate rows, their 16 up rows, per quarter
               load_tile(dst + i * 2048, &p.codes, span * 128, row + (i >> 1) * 16 + (i & 1) * n_out,
-                        &c_full[slot]);
+                        bar_c + 16 * slot);
           } else {
-            load_tile(dst, &p.codes, span * 128, row, &c_full[slot]);
+            load_tile(dst, &p.codes, span * 128, row, bar_c + 16 * slot);
           }
           ++issued;
           if (++slot == kSlots) {
@@ -597,66 +667,59 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       for (int i = min(issued, kSlots); i > 0; --i) {
         slot = slot ? slot - 1 : kSlots - 1;
         if (slot == kSlots - 1) ph ^= 1;
-        wait(&c_full[slot], ph ^ 1, a.status, 70);
+        wait_one(bar_c + 16 * slot, ph ^ 1, a.status, 70);
       }
     }
-  } else if (warp == 16) {
+  } else if (warp == 0) {
     // ------------------------------------------------------------------ MMA issuer
-    // The warp stays converged and one elected lane issues, so that descriptors are computed
-    // in uniform registers (measured: a single-lane branch spends 75 clocks per MMA).
+    // One thread and as few instructions as it takes: an MMA or a commit takes it 44 clocks.
     constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
-    const uint64_t desc0 = tc::sdesc_sw128(smem_u32(smem), 16, 1024);
-    const uint32_t half16 = (uint32_t)half_bytes >> 4;  // in descriptor units of 16 bytes
-    const uint32_t taddr = __shfl_sync(0xffffffffu, tmem, 0);
-    int st = 0, tile = 0;
-    uint32_t ph = 0, gs = 0;
-    while (cur.valid() && ok) {
-      const int rows = __shfl_sync(0xffffffffu, cur.row1() - cur.row0(), 0);
-      const uint32_t idesc = tc::idesc_f16(kBf, 128, 0, false, false) +
-                             ((uint32_t)((rows + 15) / 16 * 2) << 17);
-      const int buf = tile & 1;
-      const uint32_t acc = taddr + buf * kMaxTok;
-      ok = __all_sync(0xffffffffu, wait(&acc_free[buf], ((tile >> 1) & 1) ^ 1, a.status, 63));
-      for (int k = 0; k < steps && ok; k += 2, ++gs) {
-        const uint32_t as = gs % kAStages;
-        ok = __all_sync(0xffffffffu, wait(&b_full[st], ph, a.status, 64) &&
-                                         wait(&a_full[as], (gs / kAStages) & 1, a.status, 65));
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t am = taddr + kACol + as * kACols;
-        const uint64_t bd = desc0 + (uint64_t)(st * 2) * half16;
-        if (elect_one()) {
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            tc::mma_ts(acc, am + s * 8, bd + s * 2, idesc, k > 0 || s > 0 ? 1u : 0u);
-          if (k + 1 < steps) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              tc::mma_ts(acc, am + 32 + s * 8, bd + half16 + s * 2, idesc, 1u);
+    if (elect_one()) {
+      const uint64_t desc = tc::sdesc_sw128(smem_u32(smem), 16, 1024);
+      const uint32_t dlo = (uint32_t)desc, dhi = (uint32_t)(desc >> 32);
+      const uint32_t dhalf = (uint32_t)half_bytes >> 4;  // descriptor units of 16 bytes
+      const uint32_t bb_end = bar_b + 16 * p.b_stages;
+      uint32_t bb = bar_b, blo = dlo;  // full barrier and descriptor of the B stage
+      uint32_t bph = 0, as = 0, aph = 0, tile = 0;
+      while (cur.valid() && ok) {
+        const int rows = cur.row1() - cur.row0();
+        const uint32_t idesc = tc::idesc_f16(kBf, 128, 0, false, false) +
+                               ((uint32_t)((rows + 15) / 16 * 2) << 17);
+        const uint32_t buf = tile & 1, acc = tmem + buf * kMaxTok;
+        ok = wait_one(bar_acc + 16 * buf + 8, ((tile >> 1) & 1) ^ 1, a.status, 63);
+        for (int k = 0; k < steps && ok; k += 2) {
+          ok = wait_one(bb, bph, a.status, 64) && wait_one(bar_a + 16 * as, aph, a.status, 65);
+          if (!ok) break;
+          tc::fence_after_sync();
+          const uint32_t am = tmem + kACol + as * kACols;
+          mma4(acc, am, blo, dhi, idesc, k > 0 ? 1u : 0u);
+          if (k + 1 < steps) mma4(acc, am + 32, blo + dhalf, dhi, idesc, 1u);
+          commit(bar_a + 16 * as + 8);
+          commit(bb + 8);
+          as ^= 1;
+          aph ^= as ^ 1;
+          bb += 16;
+          blo += 2 * dhalf;
+          if (bb == bb_end) {
+            bb = bar_b;
+            blo = dlo;
+            bph ^= 1;
           }
-          tc::mma_commit(&a_free[as]);
-          tc::mma_commit(&b_free[st]);
-          if (k + 2 >= steps) tc::mma_commit(&acc_full[buf]);
         }
-        __syncwarp();
-        if (++st == p.b_stages) {
-          st = 0;
-          ph ^= 1;
-        }
+        if (ok) commit(bar_acc + 16 * buf);
+        ++tile;
+        cur.next();
       }
-      ++tile;
-      cur.next();
+      // every MMA has completed before tensor memory is freed
+      commit(bar_fin);
+      wait_one(bar_fin, 0, a.status, 66);
     }
-    // every MMA has completed before tensor memory is freed (the elected lane is the same each
-    // time, so its commits cover all of them)
-    if (elect_one()) tc::mma_commit(&mma_fin);
     __syncwarp();
-    wait(&mma_fin, 0, a.status, 66);
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (warp == 16) tc::tmem_dealloc(tmem, 512);
+  if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
 size_t smem_bytes(int E) {
