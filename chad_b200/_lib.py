@@ -78,7 +78,7 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
          _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp],
     ),
-    "qkv_matmul_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "qkv_matmul_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
     "qkv_quantized_matmul": (
         _i,
         [_vp, _ll, _vp, _vp, _vp, _vp,  # x ldx w scales biases out

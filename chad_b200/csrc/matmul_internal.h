@@ -30,7 +30,9 @@ struct MatmulArgs {
 int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st);  // few rows per weight matrix
 int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st);    // many (tcgen05)
 bool matmul_tc_fits(int E, int N);  // whether the tcgen05 kernel takes the stacked weights
+size_t matmul_tc_workspace(int R, int K);  // when it gathers rows of x
 int launch_matmul(const MatmulArgs& a, cudaStream_t st);       // whichever is faster
+bool matmul_takes_tc(int R, int E, int N);
 
 struct RouteArgs {
   const void* logits;  // (T, E) in dtype

@@ -477,7 +477,7 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
   a.K = K;
   a.dtype = dtype;
   a.act = act;
-  const size_t need = qkv_matmul_workspace_size(R, E, N, K, dtype, act);
+  const size_t need = qkv_matmul_workspace_size(R, E, N, K, rows != nullptr);
   if (need && (!workspace || ws_bytes < need))
     return fail(QKV_EWORKSPACE, "workspace %zu bytes < required %zu", ws_bytes, need);
   if (need && !aligned16(workspace)) return fail(QKV_EALIGN, "workspace must be 16-byte aligned");
@@ -489,14 +489,9 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
 
 }  // namespace
 
-size_t qkv_matmul_workspace_size(int M, int E, int N, int K, int dtype, int act) {
-  (void)M;
-  (void)E;
-  (void)N;
-  (void)K;
-  (void)dtype;
-  (void)act;
-  return 0;
+size_t qkv_matmul_workspace_size(int R, int E, int N, int K, int gathered) {
+  if (R <= 0 || E <= 0 || N <= 0 || K <= 0 || !gathered) return 0;
+  return matmul_takes_tc(R, E, N) ? matmul_tc_workspace(R, K) : 0;
 }
 
 int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void* scales,

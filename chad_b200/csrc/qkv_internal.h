@@ -123,7 +123,7 @@ bool make_code_map_bytes(CUtensorMap* m, const void* base, int RB, int NP, long 
 
 
 // Tiled tensor map over `rows` rows of `inner` elements (1 or 2 bytes), box (box_inner,
-// box_rows) with box_inner spanning 128 bytes, 128-byte swizzle.
+// box_rows) with box_inner spanning 64 or 128 bytes, swizzled by that span.
 bool make_rows_map(CUtensorMap* m, const void* base, int elem_bytes, long long inner,
                    long long rows, long long row_bytes, int box_inner, int box_rows);
 

@@ -12,9 +12,9 @@
 //     an expert's rows are cut into equal tiles. Every CTA takes a contiguous range of the
 //     tiles of equal summed cost, computed by each CTA from the offsets: nothing is counted
 //     through memory, and neighbouring tiles share rows of x in L2.
-//   * Warps: 0 issues the MMAs, 1 loads rows of x (TMA), 2 packed codes (TMA), 4-11
-//     dequantize (two warpgroups, alternate 128 K values), 12-15 store results; 1, 3 and 16-19
-//     gather rows of x (TMA, four rows a load).
+//   * Warps: 0 issues the MMAs, 1 loads rows of x (TMA), 2 packed codes (TMA), 3 scales, 4-19
+//     dequantize (four warpgroups: the two halves of 128 K values, two such in turn), 20-23
+//     store results.
 //   * Tensor memory: two accumulators of 192 columns (a tile's results are stored while the
 //     next one accumulates) and four A stages of 32 columns (64 K values each).
 //   * Gated activation: 16 gate rows and the 16 up rows of the same outputs share a warp's 32
@@ -38,25 +38,27 @@ namespace qkv {
 
 namespace {
 
-constexpr int kWarps = 20;
+constexpr int kWarps = 24;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxTok = 192;           // rows of x in a tile
-constexpr int kAStages = 2;            // of 128 K values, in tensor memory
-constexpr int kACols = 64;             // columns of an A stage
+constexpr int kAStages = 4;            // of 64 K values, in tensor memory
 constexpr int kACol = 2 * kMaxTok;     // first A column
 constexpr int kMaxBStages = 8;         // of 128 K values
 constexpr int kBBytes = 144 * 1024;    // shared memory of the B stages
-constexpr int kSlots = 4;              // prefetched spans of packed codes
-constexpr int kSlotBytes = 128 * 128;  // 128 weight rows x 128 bytes: 256 K values
+constexpr int kSlots = 4;              // prefetched stages of packed codes, two per turn
+constexpr int kSlotBytes = 128 * 64;   // 128 weight rows x 64 bytes: 128 K values
+constexpr int kScaleGroups = 16;       // groups of a staged piece of scales and biases
+constexpr int kScalePitch = 48;        // bytes of a row of a piece
+constexpr int kScaleBytes = 2 * 128 * kScalePitch;  // one piece: 128 rows of both
 // barriers, in shared memory: pairs of full and free by stage
-constexpr int kBarA = 0, kBarB = kBarA + 2 * kAStages, kBarC = kBarB + 2 * kMaxBStages;
-constexpr int kBarAcc = kBarC + 2 * kSlots, kBarFin = kBarAcc + 4, kBars = kBarFin + 1;
-constexpr int kGatherWarps = 6;        // warps 1, 3 and 16-19
+constexpr int kBarA = 0, kBarFreed = kBarA + kAStages, kBarB = kBarFreed + kAStages, kBarC = kBarB + 2 * kMaxBStages,
+              kBarS = kBarC + 2 * kSlots;
+constexpr int kBarAcc = kBarS + 4, kBarFin = kBarAcc + 4, kBars = kBarFin + 1;
 constexpr int kMaxExperts = 1024;
 
 struct TcArgs {
   CUtensorMap codes;  // (E * N, K/2) bytes; boxes of 128 rows, or of 16 gate or up rows
-  CUtensorMap x;      // (x_rows, K); boxes of `tok` rows, or single rows for gathering
+  CUtensorMap x;      // (x_rows, K); boxes of `tok` rows
   MatmulArgs a;
   int tok;       // most rows of x per tile (a multiple of 16)
   int b_stages;
@@ -122,35 +124,23 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(bar)
       : "memory");
 }
-// Scale loads, volatile so that they stay ahead of the span they are loaded under.
-__device__ __forceinline__ uint32_t ld_u16(const uint16_t* p) {
+// a 16-bit value in both halves
+__device__ __forceinline__ uint32_t lds_u16x2(uint32_t at) {
   uint16_t v;
-  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
-  return v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v * 0x10001u;
 }
-__device__ __forceinline__ uint32_t ld_u32(const uint16_t* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ void ld_v4(const uint16_t* p, uint32_t (&v)[4]) {
-  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+__device__ __forceinline__ void lds_v4(uint32_t at, uint32_t* v) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-               : "l"(p));
+               : "r"(at)
+               : "memory");
 }
-__device__ __forceinline__ bool bad_row(const MatmulArgs& a, int r) {
-  const int i = __ldg(a.rows + r);
-  return i < 0 || i >= a.x_rows;
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// four rows of `map` (any indices inside it) at a column
-__device__ __forceinline__ void load_rows4(uint32_t dst, const CUtensorMap* map, int col,
-                                           const int4& r, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w),
-      "r"(bar)
-      : "memory");
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
@@ -173,6 +163,17 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// a poll that never suspends
+__device__ __forceinline__ uint32_t test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status, int where) {
   unsigned long long t0 = 0;
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
@@ -193,14 +194,18 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, int* statu
   flag_device_error(status, where);
   return false;
 }
-// one thread
-__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, int* status, int where) {
-  return poll(bar, parity) || wait_long(bar, parity, status, where);
-}
 // a converged warp, which stays converged
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status, int where) {
   if (__all_sync(0xffffffffu, poll(bar, parity))) return true;
   return __all_sync(0xffffffffu, wait_long(bar, parity, status, where));
+}
+// three barriers, their polls in flight together
+__device__ __forceinline__ bool wait_three(uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
+                                           uint32_t b3, uint32_t p3, int* status, int where) {
+  const bool r1 = poll(b1, p1), r2 = poll(b2, p2), r3 = poll(b3, p3);
+  if (__all_sync(0xffffffffu, r1 & r2 & r3)) return true;
+  return wait_warp(b1, p1, status, where) && wait_warp(b2, p2, status, where + 10) &&
+         wait_warp(b3, p3, status, where + 11);
 }
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar)
@@ -240,7 +245,7 @@ struct Cursor {
   int cost, row_begin, row_end;
 
   __device__ __forceinline__ void set_expert() {
-    const int lo = off[e], hi = off[e + 1];
+    const int lo = __shfl_sync(0xffffffffu, off[e], 0), hi = __shfl_sync(0xffffffffu, off[e + 1], 0);
     row_begin = lo;
     row_end = hi;
     s = split_rows(hi - lo, tok);
@@ -264,8 +269,7 @@ struct Cursor {
   }
 };
 
-// SB: how scales are read (0 singly, 1 in pairs, 2 eight at a time)
-template <typename T, bool GATED, int SB>
+template <typename T, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_constant__ TcArgs p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t bars[kBars];
@@ -275,23 +279,30 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   const MatmulArgs& a = p.a;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* codes = smem + kBBytes;
-  int* off = (int*)(codes + kSlots * kSlotBytes);  // E + 1 clamped offsets
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* scales = codes + kSlots * kSlotBytes;     // two pieces
+  int* off = (int*)(scales + 2 * kScaleBytes);       // E + 1 clamped offsets
+  // broadcast, so that the compiler knows it for uniform: every branch it takes for divergent
+  // costs over a hundred clocks of convergence bookkeeping (measured)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int steps = a.K / 64;  // K steps of one group
 
   // ---- set-up: barriers, tensor memory, this CTA's range of tiles --------------------------
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAStages; ++i) {
-      mbar_init(&bars[kBarA + 2 * i], 4);
-      mbar_init(&bars[kBarA + 2 * i + 1], 1);
+      mbar_init(&bars[kBarA + i], 4);
+      mbar_init(&bars[kBarFreed + i], 1);
     }
     for (int i = 0; i < kMaxBStages; ++i) {
-      mbar_init(&bars[kBarB + 2 * i], a.rows ? kGatherWarps : 1);
+      mbar_init(&bars[kBarB + 2 * i], 1);
       mbar_init(&bars[kBarB + 2 * i + 1], 1);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars[kBarC + 2 * i], 1);
       mbar_init(&bars[kBarC + 2 * i + 1], 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[kBarS + 2 * i], 32);
+      mbar_init(&bars[kBarS + 2 * i + 1], 16);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[kBarAcc + 2 * i], 1);
@@ -362,147 +373,92 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   cur.E = a.E;
   cur.tok = p.tok;
   cur.n_tiles = p.n_tiles;
-  cur.e = start_sh[0];
-  cur.seg = start_sh[1];
-  cur.j = start_sh[2];
-  cur.pos = range_sh[0];
-  cur.end = range_sh[1];
+  cur.e = __shfl_sync(0xffffffffu, start_sh[0], 0);
+  cur.seg = __shfl_sync(0xffffffffu, start_sh[1], 0);
+  cur.j = __shfl_sync(0xffffffffu, start_sh[2], 0);
+  cur.pos = __shfl_sync(0xffffffffu, range_sh[0], 0);
+  cur.end = __shfl_sync(0xffffffffu, range_sh[1], 0);
   if (cur.e < a.E) cur.set_expert();
   const int n_out = GATED ? a.N / 2 : a.N;
+  // weight row of row r of tile j (clamped into the matrix; what is past it is not stored)
+  auto weight_row = [&](int e, int j, int r) -> long long {
+    const int n = GATED ? min(j * 64 + (r >> 5) * 16 + (r & 15), n_out - 1) + (r >> 4 & 1) * n_out
+                        : min(j * 128 + r, n_out - 1);
+    return (long long)e * a.N + n;
+  };
   const int half_bytes = p.tok * 128;  // a B stage is two tiles of 64 K values
-  // full barrier of A stage i at bar_a + 16 i, its free barrier 8 bytes on; the others alike
-  const uint32_t bar_a = smem_u32(bars), bar_b = bar_a + 8 * kBarB, bar_c = bar_a + 8 * kBarC;
-  const uint32_t bar_acc = bar_a + 8 * kBarAcc, bar_fin = bar_a + 8 * kBarFin;
+  // full barrier of B stage i at bar_b + 16 i, its free barrier 8 bytes on; the others alike.
+  // A double step (128 K values) has a turn, 0 or 1 in alternation from every tile's first: two
+  // A stages (one per half; full barriers by stage, freed barriers by turn), two warpgroups and
+  // two stages of codes, which count the double steps of their turn.
+  const uint32_t bar_a = smem_u32(bars), bar_freed = bar_a + 8 * kBarFreed, bar_b = bar_a + 8 * kBarB, bar_c = bar_a + 8 * kBarC;
+  const uint32_t bar_s = bar_a + 8 * kBarS, bar_acc = bar_a + 8 * kBarAcc, bar_fin = bar_a + 8 * kBarFin;
   bool ok = true;
 
-  if (warp >= 4 && warp < 12) {
+  if (warp >= 4 && warp < 20) {
     // ------------------------------------------------------------------ dequantizers
-    const int par = (warp >> 2) - 1, q = warp & 3;  // double step of a span; tensor memory lanes 32q..32q+31
-    const int spans = (steps + 3) / 4;
-    const uint32_t my_row = smem_u32(codes) + (q * 32 + lane) * 128;
-    int slot = 0;
-    uint32_t ph = 0;
-    uint32_t gs = 0;  // double steps of all tiles so far: A stage gs % 2
+    // half h of the double steps of a turn; tensor memory lanes 32q..32q+31
+    const int h = (warp >> 2) - 1 & 1, turn = (warp >> 2) - 1 >> 1, q = warp & 3;
+    const uint32_t my_row = smem_u32(codes) + turn * 2 * kSlotBytes + (q * 32 + lane) * 64;
+    const uint32_t at0 = my_row + (((2 * h) ^ (lane >> 1 & 3)) << 4);
+    const uint32_t at1 = my_row + (((2 * h + 1) ^ (lane >> 1 & 3)) << 4);
+    const uint32_t my_scales =
+        smem_u32(scales) + (q * 32 + lane) * kScalePitch + (2 * turn + h) * 2;
+    const uint32_t my_a = tmem + kACol + turn * 64 + h * 32 + ((uint32_t)(q * 32) << 16);
+    const uint32_t my_full = bar_a + 8 * (turn * 2 + h), my_freed = bar_freed + 8 * turn;
+    const uint32_t my_codes = bar_c + 32 * turn;
+    const bool one = lane == 0;
+    uint32_t n = 0, piece = 0;  // double steps of this turn, pieces of scales so far
     while (cur.valid() && ok) {
-      // weight row of this lane (clamped into the matrix; what is past it is not stored)
-      const int wn = GATED ? min(cur.j * 64 + q * 16 + (lane & 15), n_out - 1) + (lane >> 4) * n_out
-                           : min(cur.j * 128 + q * 32 + lane, n_out - 1);
-      const long long wr = (long long)cur.e * a.N + wn;
-      const uint16_t* sp = (const uint16_t*)a.scales + wr * steps;
-      const uint16_t* bp = (const uint16_t*)a.biases + wr * steps;
-      // scales and biases: pairs for this warpgroup's two K steps of a span, loaded a span (or
-      // two, sixteen bytes at a time) ahead; a lane reads its own row, so wide loads save L1
-      uint32_t cs[4], cb[4], ns[4], nb[4];
-      auto load_sb = [&](int span) {
-        const int k = span * 4;
-        if (SB == 2) {
-          if (k < steps) {
-            ld_v4(sp + k, ns);
-            ld_v4(bp + k, nb);
-          }
-        } else if (SB == 1) {
-          if (k + 2 * par < steps) {
-            ns[0] = ld_u32(sp + k + 2 * par);
-            nb[0] = ld_u32(bp + k + 2 * par);
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int kk = min(k + 2 * par + h, steps - 1);
-            ns[h] = ld_u16(sp + kk);
-            nb[h] = ld_u16(bp + kk);
-          }
-        }
-      };
-      load_sb(0);
-      for (int span = 0; span < spans && ok; ++span) {
-        uint32_t s2[2], b2[2];  // scale and bias of each step in both halves
-        if (SB == 2) {
-          if (!(span & 1)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              cs[i] = ns[i];
-              cb[i] = nb[i];
-            }
-            load_sb(span + 2);
-          }
-          const uint32_t sw = span & 1 ? (par ? cs[3] : cs[2]) : (par ? cs[1] : cs[0]);
-          const uint32_t bw = span & 1 ? (par ? cb[3] : cb[2]) : (par ? cb[1] : cb[0]);
-          s2[0] = prmt(sw, sw, 0x1010), s2[1] = prmt(sw, sw, 0x3232);
-          b2[0] = prmt(bw, bw, 0x1010), b2[1] = prmt(bw, bw, 0x3232);
-        } else if (SB == 1) {
-          s2[0] = prmt(ns[0], ns[0], 0x1010), s2[1] = prmt(ns[0], ns[0], 0x3232);
-          b2[0] = prmt(nb[0], nb[0], 0x1010), b2[1] = prmt(nb[0], nb[0], 0x3232);
-          if (span + 1 < spans) load_sb(span + 1);
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            s2[h] = prmt(ns[h], ns[h], 0x1010);
-            b2[h] = prmt(nb[h], nb[h], 0x1010);
-          }
-          if (span + 1 < spans) load_sb(span + 1);
-        }
-        ok = wait_warp(bar_c + 16 * slot, ph, a.status, 67);
+      for (int k0 = 0; k0 < steps; k0 += kScaleGroups, ++piece) {
+        const uint32_t s_bar = bar_s + 16 * (piece & 1);
+        uint32_t sat = my_scales + (piece & 1) * kScaleBytes;
+        ok = wait_warp(s_bar, piece >> 1 & 1, a.status, 71);
         if (!ok) break;
-        const int k0 = span * 4 + 2 * par;  // this warpgroup's steps k0 and k0 + 1
-        if (k0 < steps) {
-          const uint32_t g = gs + span * 2 + par, st = g % kAStages;
-          const uint32_t dst = tmem + kACol + st * kACols + ((uint32_t)(q * 32) << 16);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t out[32];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t wv[4];
-              const uint32_t at = my_row + slot * kSlotBytes +
-                                  (((4 * par + 2 * h + i) ^ (lane & 7)) << 4);
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(wv[0]), "=r"(wv[1]), "=r"(wv[2]), "=r"(wv[3])
-                           : "r"(at)
-                           : "memory");
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                uint32_t v[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  v[c] = Conv<T>::fma(
-                      Conv<T>::sub(and_or(wv[w] >> (4 * c), 0x000f000fu, Conv<T>::kMagic)), s2[h],
-                      b2[h]);
-                // (0,4)(1,5)(2,6)(3,7) -> (0,1)(2,3)(4,5)(6,7)
-                out[16 * i + 4 * w + 0] = prmt(v[0], v[1], 0x5410);
-                out[16 * i + 4 * w + 1] = prmt(v[2], v[3], 0x5410);
-                out[16 * i + 4 * w + 2] = prmt(v[0], v[1], 0x7632);
-                out[16 * i + 4 * w + 3] = prmt(v[2], v[3], 0x7632);
-              }
-            }
-            // the first half is converted before the stage is free
-            if (h == 0) {
-              ok = wait_warp(bar_a + 16 * st + 8, ((g / kAStages) & 1) ^ 1, a.status, 60);
-              if (!ok) break;
-              tc::fence_after_sync();
-            }
-            // (the second half of an odd last step holds zeros that no MMA reads)
-            tc::st32(dst + h * 32, out);
-          }
+#pragma unroll 1
+        for (int k = k0 + 2 * turn; k < min(k0 + kScaleGroups, steps); k += 4, ++n, sat += 8) {
+          // (half 1 of an odd last step converts what is not multiplied, to keep the count)
+          const uint32_t slot = n & 1;
+          ok = wait_warp(my_codes + 16 * slot, n >> 1 & 1, a.status, 67);
           if (!ok) break;
+          const uint32_t s2 = lds_u16x2(sat), b2 = lds_u16x2(sat + 128 * kScalePitch);
+          uint32_t out[32], wv[8];
+          lds_v4(at0 + slot * kSlotBytes, wv);
+          lds_v4(at1 + slot * kSlotBytes, wv + 4);
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            // byte c of a word holds codes 2c and 2c + 1: its low nibble and, from the word
+            // shifted by four, its high one go to the two halves
+            const uint32_t up = wv[w] >> 4;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t pair = prmt(wv[w], up, 0x0400u + 0x0101u * c);
+              out[4 * w + c] =
+                  Conv<T>::fma(Conv<T>::sub(and_or(pair, 0x000f000fu, Conv<T>::kMagic)), s2, b2);
+            }
+          }
+          // converted before the stage is free, so that it is stored at once
+          ok = wait_warp(my_freed, (n & 1) ^ 1, a.status, 60);
+          if (!ok) break;
+          tc::fence_after_sync();
+          tc::st32(my_a, out);
           tc::wait_st();
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) arrive(bar_a + 16 * st);
+          // the codes are freed after their last use, not after their loads: a load that the
+          // assembler moved below the arrive would read the stage's next contents
+          if (one) {
+            arrive(my_full);
+            arrive(my_codes + 16 * slot + 8);
+          }
         }
-        // after the last use of the words, not after their loads: a load that the assembler
-        // moved below this arrive would read the slot's next contents
+        if (!ok) break;
         __syncwarp();
-        if (lane == 0) arrive(bar_c + 16 * slot + 8);
-        if (++slot == kSlots) {
-          slot = 0;
-          ph ^= 1;
-        }
+        if (one) arrive(s_bar + 8);
       }
-      gs += (steps + 1) / 2;
       cur.next();
     }
-  } else if (warp >= 12 && warp < 16) {
+  } else if (warp >= 20) {
     // ------------------------------------------------------------------ results
     const int q = warp & 3;
     int tile = 0;
@@ -516,19 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       const int n = GATED ? cur.j * 64 + q * 16 + (lane & 15) : cur.j * 128 + q * 32 + lane;
       const uint32_t acc = tmem + buf * kMaxTok + ((uint32_t)(q * 32) << 16);
       T* o = out + (long long)row0 * n_out + n;
-      bool bad = false;  // whether a row of the tile has an index outside x
-      if (a.rows)
-        for (int t = lane; t < rows; t += 32) bad |= bad_row(a, row0 + t);
-      bad = __any_sync(0xffffffffu, bad);
       for (int c0 = 0; c0 < rows; c0 += 16) {
         uint32_t r[16];
         tc::ld16(acc + c0, r);
         tc::wait_ld();
-        if (bad) {
-#pragma unroll
-          for (int c = 0; c < 16; ++c)
-            if (c0 + c < rows && bad_row(a, row0 + c0 + c)) r[c] = 0;
-        }
         const bool full = c0 + 16 <= rows;
         if (GATED) {
           const bool hi = lane >= 16;  // lanes 0-15 finish column c, lanes 16-31 column c + 1
@@ -558,68 +505,90 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       ++tile;
       cur.next();
     }
-  } else if (warp == 1 && !a.rows) {
-    // ------------------------------------------------------------------ rows of x, in order
-    if (lane == 0) {
-      const uint32_t base = smem_u32(smem);
-      int st = 0, issued = 0;
-      uint32_t ph = 1;
-      while (cur.valid() && ok) {
-        const int row0 = cur.row0();
-        for (int k = 0; k < steps; k += 2) {
-          ok = wait_one(bar_b + 16 * st + 8, ph, a.status, 62);
-          if (!ok) break;
-          const uint32_t dst = base + st * 2 * half_bytes;
-          arrive_tx(bar_b + 16 * st, k + 1 < steps ? 2 * half_bytes : half_bytes);
-          load_tile(dst, &p.x, k * 64, row0, bar_b + 16 * st);
-          if (k + 1 < steps) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar_b + 16 * st);
-          ++issued;
-          if (++st == p.b_stages) {
-            st = 0;
-            ph ^= 1;
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ scales and biases
+    // A dequantizer lane reading its own row from global memory would cost the load pipe a
+    // lookup per lane and stall its warp (34 clocks per load, measured), so this warp stages
+    // pieces of 16 groups of the tile's 128 rows.
+    const uint32_t base = smem_u32(scales);
+    const uintptr_t bits = (uintptr_t)a.scales | (uintptr_t)a.biases;
+    const bool wide = steps % 8 == 0 && bits % 16 == 0, pairs = steps % 2 == 0 && bits % 4 == 0;
+    uint32_t buf = 0, ph = 1;
+    while (cur.valid() && ok) {
+      for (int g0 = 0; g0 < steps; g0 += kScaleGroups) {
+        ok = wait_warp(bar_s + 16 * buf + 8, ph, a.status, 72);
+        if (!ok) break;
+        const uint32_t dst = base + buf * kScaleBytes;
+        const uint16_t* const arrays[2] = {(const uint16_t*)a.scales, (const uint16_t*)a.biases};
+        if (wide) {
+          const int g = g0 + (lane & 1) * 8;
+#pragma unroll 4
+          for (int i = 0; i < 8; ++i) {
+            const int r = (lane >> 1) + 16 * i;
+            const long long at = weight_row(cur.e, cur.j, r) * steps + g;
+            if (g < steps) {
+              cp16(dst + r * kScalePitch + (lane & 1) * 16, arrays[0] + at);
+              cp16(dst + (128 + r) * kScalePitch + (lane & 1) * 16, arrays[1] + at);
+            }
+          }
+        } else if (pairs) {
+          const int g = g0 + (lane & 7) * 2;
+#pragma unroll 8
+          for (int i = 0; i < 32; ++i) {
+            const int r = (lane >> 3) + 4 * i;
+            const long long at = weight_row(cur.e, cur.j, r) * steps + g;
+            if (g < steps) {
+              cp4(dst + r * kScalePitch + (lane & 7) * 4, arrays[0] + at);
+              cp4(dst + (128 + r) * kScalePitch + (lane & 7) * 4, arrays[1] + at);
+            }
+          }
+        } else {
+          const int g = min(g0 + (lane & 15), steps - 1);
+#pragma unroll 1
+          for (int i0 = 0; i0 < 64; i0 += 16) {
+            uint16_t v[2][16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const long long at = weight_row(cur.e, cur.j, (lane >> 4) + 2 * (i0 + i)) * steps + g;
+              v[0][i] = __ldg(arrays[0] + at);
+              v[1][i] = __ldg(arrays[1] + at);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t to = dst + ((lane >> 4) + 2 * (i0 + i)) * kScalePitch + (lane & 15) * 2;
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v[0][i]) : "memory");
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 128 * kScalePitch), "h"(v[1][i])
+                           : "memory");
+            }
           }
         }
-        cur.next();
+        if (wide || pairs)  // when the copies have landed
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_s + 16 * buf)
+                       : "memory");
+        else
+          arrive(bar_s + 16 * buf);
+        buf ^= 1;
+        ph ^= buf ^ 1;
       }
-      // no copy is in flight when the CTA exits, not even after a wait that gave up
-      for (int i = min(issued, p.b_stages); i > 0; --i) {
-        st = st ? st - 1 : p.b_stages - 1;
-        if (st == p.b_stages - 1) ph ^= 1;
-        wait_one(bar_b + 16 * st, ph ^ 1, a.status, 68);
-      }
+      cur.next();
     }
-  } else if (a.rows && (warp == 1 || warp == 3 || warp >= 16)) {
-    // ------------------------------------------------------------------ rows of x, gathered
-    // four rows per load; a load instruction takes a thread about 44 clocks, so six warps
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ rows of x, in order
     const uint32_t base = smem_u32(smem);
-    const int w = warp < 16 ? warp >> 1 : warp - 14;
     int st = 0, issued = 0;
     uint32_t ph = 1;
     while (cur.valid() && ok) {
-      const int row0 = cur.row0(), row1 = cur.row1();
-      const int n4 = (row1 - row0 + 15) / 16 * 4;
-      const int four = w + kGatherWarps * lane;
-      const int mine = (n4 - w + kGatherWarps - 1) / kGatherWarps;  // fours of this warp
-      int4 idx = make_int4(0, 0, 0, 0);  // (bad and missing rows load row 0)
-      if (four < n4) {
-        int v[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int r = row0 + four * 4 + c;
-          v[c] = r < row1 ? a.rows[r] : 0;
-          if (v[c] < 0 || v[c] >= a.x_rows) v[c] = 0;
-        }
-        idx = make_int4(v[0], v[1], v[2], v[3]);
-      }
+      const int row0 = cur.row0();
       for (int k = 0; k < steps; k += 2) {
         ok = wait_warp(bar_b + 16 * st + 8, ph, a.status, 62);
         if (!ok) break;
-        const uint32_t dst = base + st * 2 * half_bytes + four * 512;
-        if (lane == 0) arrive_tx(bar_b + 16 * st, mine * (k + 1 < steps ? 1024 : 512));
-        __syncwarp();
-        if (four < n4) {
-          load_rows4(dst, &p.x, k * 64, idx, bar_b + 16 * st);
-          if (k + 1 < steps) load_rows4(dst + half_bytes, &p.x, k * 64 + 64, idx, bar_b + 16 * st);
+        const uint32_t dst = base + st * 2 * half_bytes, bar = bar_b + 16 * st;
+        const bool both = k + 1 < steps;
+        if (elect_one()) {
+          arrive_tx(bar, both ? 2 * half_bytes : half_bytes);
+          load_tile(dst, &p.x, k * 64, row0, bar);
+          if (both) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar);
         }
         ++issued;
         if (++st == p.b_stages) {
@@ -629,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       }
       cur.next();
     }
+    // no copy is in flight when the CTA exits, not even after a wait that gave up
     for (int i = min(issued, p.b_stages); i > 0; --i) {
       st = st ? st - 1 : p.b_stages - 1;
       if (st == p.b_stages - 1) ph ^= 1;
@@ -636,85 +606,98 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ packed codes
-    if (lane == 0) {
-      const uint32_t base = smem_u32(codes);
-      const int spans = (steps + 3) / 4;
-      int slot = 0, issued = 0;
-      uint32_t ph = 1;
-      while (cur.valid() && ok) {
-        const int row = cur.e * a.N + cur.j * (GATED ? 64 : 128);
-        for (int span = 0; span < spans; ++span) {
-          ok = wait_one(bar_c + 16 * slot + 8, ph, a.status, 69);
-          if (!ok) break;
-          const uint32_t dst = base + slot * kSlotBytes;
-          arrive_tx(bar_c + 16 * slot, kSlotBytes);
-          if (GATED) {
+    const uint32_t base = smem_u32(codes);
+    uint32_t n[2] = {0, 0};  // double steps of either turn so far
+    while (cur.valid() && ok) {
+      const int row = cur.e * a.N + cur.j * (GATED ? 64 : 128);
+      for (int k = 0; k < steps && ok; k += 4) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)  // 16 gate rows, their 16 up rows, per quarter
-              load_tile(dst + i * 2048, &p.codes, span * 128, row + (i >> 1) * 16 + (i & 1) * n_out,
-                        bar_c + 16 * slot);
-          } else {
-            load_tile(dst, &p.codes, span * 128, row, bar_c + 16 * slot);
-          }
-          ++issued;
-          if (++slot == kSlots) {
-            slot = 0;
-            ph ^= 1;
+        for (int turn = 0; turn < 2; ++turn) {
+          const int kk = k + 2 * turn;
+          if (kk < steps && ok) {
+            const uint32_t slot = turn * 2 + (n[turn] & 1);
+            const uint32_t dst = base + slot * kSlotBytes, bar = bar_c + 16 * slot;
+            ok = wait_warp(bar + 8, (n[turn] >> 1 & 1) ^ 1, a.status, 69);
+            if (ok) {
+              if (elect_one()) {
+                arrive_tx(bar, kSlotBytes);
+                if (GATED) {
+#pragma unroll
+                  for (int i = 0; i < 8; ++i)  // 16 gate rows, their 16 up rows, per quarter
+                    load_tile(dst + i * 1024, &p.codes, kk * 32,
+                              row + (i >> 1) * 16 + (i & 1) * n_out, bar);
+                } else {
+                  load_tile(dst, &p.codes, kk * 32, row, bar);
+                }
+              }
+              ++n[turn];
+            }
           }
         }
-        cur.next();
       }
-      for (int i = min(issued, kSlots); i > 0; --i) {
-        slot = slot ? slot - 1 : kSlots - 1;
-        if (slot == kSlots - 1) ph ^= 1;
-        wait_one(bar_c + 16 * slot, ph ^ 1, a.status, 70);
-      }
+      cur.next();
     }
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn)
+      for (uint32_t i = n[turn] < 2 ? 0 : n[turn] - 2; i < n[turn]; ++i)
+        wait_warp(bar_c + 16 * (turn * 2 + (i & 1)), i >> 1 & 1, a.status, 70);
   } else if (warp == 0) {
     // ------------------------------------------------------------------ MMA issuer
-    // One thread and as few instructions as it takes: an MMA or a commit takes it 44 clocks.
+    // As few instructions as it takes: an MMA or a commit takes its thread 44 clocks.
     constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
-    if (elect_one()) {
-      const uint64_t desc = tc::sdesc_sw128(smem_u32(smem), 16, 1024);
-      const uint32_t dlo = (uint32_t)desc, dhi = (uint32_t)(desc >> 32);
-      const uint32_t dhalf = (uint32_t)half_bytes >> 4;  // descriptor units of 16 bytes
-      const uint32_t bb_end = bar_b + 16 * p.b_stages;
-      uint32_t bb = bar_b, blo = dlo;  // full barrier and descriptor of the B stage
-      uint32_t bph = 0, as = 0, aph = 0, tile = 0;
-      while (cur.valid() && ok) {
-        const int rows = cur.row1() - cur.row0();
-        const uint32_t idesc = tc::idesc_f16(kBf, 128, 0, false, false) +
-                               ((uint32_t)((rows + 15) / 16 * 2) << 17);
-        const uint32_t buf = tile & 1, acc = tmem + buf * kMaxTok;
-        ok = wait_one(bar_acc + 16 * buf + 8, ((tile >> 1) & 1) ^ 1, a.status, 63);
-        for (int k = 0; k < steps && ok; k += 2) {
-          ok = wait_one(bb, bph, a.status, 64) && wait_one(bar_a + 16 * as, aph, a.status, 65);
-          if (!ok) break;
-          tc::fence_after_sync();
-          const uint32_t am = tmem + kACol + as * kACols;
-          mma4(acc, am, blo, dhi, idesc, k > 0 ? 1u : 0u);
-          if (k + 1 < steps) mma4(acc, am + 32, blo + dhalf, dhi, idesc, 1u);
-          commit(bar_a + 16 * as + 8);
-          commit(bb + 8);
-          as ^= 1;
-          aph ^= as ^ 1;
-          bb += 16;
-          blo += 2 * dhalf;
-          if (bb == bb_end) {
-            bb = bar_b;
-            blo = dlo;
-            bph ^= 1;
-          }
+    const uint64_t desc = tc::sdesc_sw128(smem_u32(smem), 16, 1024);
+    const uint32_t dlo = (uint32_t)desc, dhi = (uint32_t)(desc >> 32);
+    const uint32_t dhalf = (uint32_t)half_bytes >> 4;  // descriptor units of 16 bytes
+    const uint32_t bb_end = bar_b + 16 * p.b_stages;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t bb = bar_b, blo = dlo;  // full barrier and descriptor of the B stage
+    uint32_t bph = 0, aph = 0, tile = 0;  // bit t of aph: phase of turn t
+    uint32_t ready = 0;  // the next double step's barriers, tested while this one's MMAs run
+    while (cur.valid() && ok) {
+      const int rows = cur.row1() - cur.row0();
+      const uint32_t idesc = tc::idesc_f16(kBf, 128, 0, false, false) +
+                             ((uint32_t)((rows + 15) / 16 * 2) << 17);
+      const uint32_t buf = tile & 1, acc = tm + buf * kMaxTok;
+      ok = wait_warp(bar_acc + 16 * buf + 8, (tile >> 1 & 1) ^ 1, a.status, 63);
+      uint32_t turn = 0;
+      for (int k = 0; k < steps && ok; k += 2) {
+        const uint32_t ba = bar_a + 16 * turn, ph = aph >> turn & 1;
+        if (!__all_sync(0xffffffffu, ready)) ok = wait_three(bb, bph, ba, ph, ba + 8, ph, a.status, 64);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const bool last = k + 2 >= steps;
+        const uint32_t am = tm + kACol + turn * 64, b_free = bb + 8, b_at = blo;
+        const uint32_t freed = bar_freed + 8 * turn;
+        aph ^= 1u << turn;
+        turn = last ? 0 : turn ^ 1;
+        bb += 16;
+        blo += 2 * dhalf;
+        if (bb == bb_end) {
+          bb = bar_b;
+          blo = dlo;
+          bph ^= 1;
         }
-        if (ok) commit(bar_acc + 16 * buf);
-        ++tile;
-        cur.next();
+        const uint32_t na = bar_a + 16 * turn, nph = aph >> turn & 1;
+        ready = 1;
+        if (elect_one()) {
+          mma4(acc, am, b_at, dhi, idesc, k > 0 ? 1u : 0u);
+          if (k + 1 < steps) mma4(acc, am + 32, b_at + dhalf, dhi, idesc, 1u);
+          // by now the stages freed by the double step before have been refilled
+          ready = test(bb, bph) & test(na, nph) & test(na + 8, nph);
+          commit(freed);
+          commit(b_free);
+          if (last) commit(bar_acc + 16 * buf);
+        }
+        __syncwarp();
       }
-      // every MMA has completed before tensor memory is freed
-      commit(bar_fin);
-      wait_one(bar_fin, 0, a.status, 66);
+      ++tile;
+      cur.next();
     }
+    // every MMA has completed before tensor memory is freed (one lane, the same each time,
+    // issued them all)
+    if (elect_one()) commit(bar_fin);
     __syncwarp();
+    wait_warp(bar_fin, 0, a.status, 66);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -722,41 +705,51 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   if (warp == 0) tc::tmem_dealloc(tmem, 512);
 }
 
-size_t smem_bytes(int E) {
-  return 1024 + kBBytes + kSlots * kSlotBytes + (size_t)(E + 1) * sizeof(int);
+// The rows of x that `rows` names, one after the other; a bad index gives a row of zeros. The
+// product kernel could gather by itself, but four-row TMA loads and 16-byte cp.async both
+// brought 32 bytes a clock and SM where its MMAs take 64 (experts-prefill sizes: 185 us with
+// gathering inside, against 15 us for this kernel and the time without).
+__global__ void __launch_bounds__(256)
+    gather_rows_kernel(const uint4* __restrict__ x, long long ldx, int x_rows,
+                       const int* __restrict__ rows, uint4* __restrict__ out, int R, int per_row) {
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= R) return;
+  const int from = rows[r];
+  const bool in = from >= 0 && from < x_rows;
+  const uint4* src = x + (in ? from : 0) * ldx;
+  uint4* dst = out + (long long)r * per_row;
+  for (int c = threadIdx.x & 31; c < per_row; c += 32)
+    dst[c] = in ? src[c] : make_uint4(0, 0, 0, 0);
 }
 
-template <typename T, bool GATED, int SB>
-int launch_tc_s(TcArgs& p, int grid, cudaStream_t st) {
+size_t smem_bytes(int E) {
+  return 1024 + kBBytes + kSlots * kSlotBytes + 2 * kScaleBytes + (size_t)(E + 1) * sizeof(int);
+}
+
+template <typename T, bool GATED>
+int launch_tc_t(TcArgs& p, int grid, cudaStream_t st) {
   const size_t smem = smem_bytes(p.a.E);
   static std::atomic<unsigned long long> ready{0};  // devices whose shared memory bound is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ECUDA;
   if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(matmul_tc_kernel<T, GATED, SB>,
+    if (cudaFuncSetAttribute(matmul_tc_kernel<T, GATED>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)smem_bytes(kMaxExperts)) != cudaSuccess)
       return QKV_ECUDA;
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
-  if (!make_rows_map(&p.codes, p.a.w, 1, p.a.K / 2, (long long)p.a.E * p.a.N, p.a.K / 2, 128,
+  if (!make_rows_map(&p.codes, p.a.w, 1, p.a.K / 2, (long long)p.a.E * p.a.N, p.a.K / 2, 64,
                      GATED ? 16 : 128) ||
-      !make_rows_map(&p.x, p.a.x, 2, p.a.K, p.a.x_rows, p.a.ldx * 2, 64, p.a.rows ? 1 : p.tok))
+      !make_rows_map(&p.x, p.a.x, 2, p.a.K, p.a.x_rows, p.a.ldx * 2, 64, p.tok))
     return QKV_ECUDA;
-  matmul_tc_kernel<T, GATED, SB><<<grid, kThreads, smem, st>>>(p);
+  matmul_tc_kernel<T, GATED><<<grid, kThreads, smem, st>>>(p);
   return QKV_OK;
 }
 
-template <typename T, bool GATED>
-int launch_tc_t(TcArgs& p, int grid, cudaStream_t st) {
-  const int groups = p.a.K / 64;
-  const uintptr_t at = (uintptr_t)p.a.scales | (uintptr_t)p.a.biases;
-  if (groups % 8 == 0 && at % 16 == 0) return launch_tc_s<T, GATED, 2>(p, grid, st);
-  if (groups % 2 == 0 && at % 4 == 0) return launch_tc_s<T, GATED, 1>(p, grid, st);
-  return launch_tc_s<T, GATED, 0>(p, grid, st);
-}
-
 }  // namespace
+
+size_t matmul_tc_workspace(int R, int K) { return (size_t)R * K * 2; }
 
 bool matmul_tc_fits(int E, int N) {
   return E <= kMaxExperts && (long long)E * N < (1ll << 31) - 256;  // 32-bit TMA coordinates
@@ -768,6 +761,14 @@ int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st) {
   const int sms = num_sms();
   TcArgs p;
   p.a = a;
+  if (a.rows) {
+    gather_rows_kernel<<<(a.R + 7) / 8, 256, 0, st>>>((const uint4*)a.x, a.ldx / 8, a.x_rows,
+                                                      a.rows, (uint4*)a.workspace, a.R, a.K / 8);
+    p.a.x = a.workspace;
+    p.a.ldx = a.K;
+    p.a.x_rows = a.R;
+    p.a.rows = nullptr;
+  }
   p.n_tiles = gated ? (n_out + 63) / 64 : (n_out + 127) / 128;
   // One matrix: the row tile that leaves the fewest idle SMs in the last wave. Experts: the
   // counts are on the device, so the largest.

@@ -421,9 +421,8 @@ def _check_out(out: torch.Tensor, shape, like: torch.Tensor) -> None:
 
 
 @functools.lru_cache(maxsize=4096)
-def _matmul_workspace_size(device: int, m: int, e: int, n: int, k: int, dt: int, act: int) -> int:
-    # the kernel choice depends on the current device's SM count: memoized per device
-    return int(_lib.load().qkv_matmul_workspace_size(m, e, n, k, dt, act))
+def _matmul_workspace_size(r: int, e: int, n: int, k: int, gathered: bool) -> int:
+    return int(_lib.load().qkv_matmul_workspace_size(r, e, n, k, 1 if gathered else 0))
 
 
 def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int = 4,
@@ -469,11 +468,9 @@ def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int
     if idx != _current_device():
         with torch.cuda.device(idx):
             return quantized_matmul(x, w_quant, bits, group_size, activation=activation, out=out)
-    need = _matmul_workspace_size(idx, m, 1, n, k, dt, act)
-    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     check(_lib.fn("qkv_quantized_matmul")(
         x.data_ptr(), ldx, w.data_ptr(), s.data_ptr(), b.data_ptr(), out.data_ptr(), m, n, k,
-        bits, group_size, dt, act, _ptr(work), need,
+        bits, group_size, dt, act, None, 0,
         _RAW_STREAM(idx) if _RAW_STREAM is not None else _stream(x.device)))
     if CHECK_EACH_CALL:
         check_device()
@@ -529,7 +526,7 @@ def grouped_quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor],
         with torch.cuda.device(idx):
             return grouped_quantized_matmul(x, w_quant, offsets, rows=rows, bits=bits,
                                             group_size=group_size, activation=activation, out=out)
-    need = _matmul_workspace_size(idx, r, e, n, k, dt, act)
+    need = _matmul_workspace_size(r, e, n, k, True) if rows is not None else 0
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     check(_lib.fn("qkv_grouped_matmul")(
         x.data_ptr(), x.stride(0) if t > 1 else k, t, _ptr(rows), offsets.data_ptr(),

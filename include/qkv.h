@@ -257,9 +257,10 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
  * QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
  * x and w 16-byte aligned, the others naturally. Non-finite x makes its own row of out
  * non-finite (inf or NaN) and no other. M = 0 does nothing.
- * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter.
+ * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter. R rows
+ * of out, E weight matrices (1 here), gathered != 0 when `rows` is given (below).
  */
-size_t qkv_matmul_workspace_size(int M, int E, int N, int K, int dtype, int act);
+size_t qkv_matmul_workspace_size(int R, int E, int N, int K, int gathered);
 int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void* scales,
                          const void* biases, void* out, int M, int N, int K, int bits,
                          int group_size, int dtype, int act, void* workspace, size_t ws_bytes,
