@@ -15,10 +15,13 @@
 // (i, i+4); the MMA sums over k, so x is paired the same way and no code moves.
 //
 // What bounds it: the packed weights, read once from HBM. A warp owns 16 weight rows and a
-// share of the K chunks (256 values, 128 bytes of each row); warps of a CTA split K until the
-// machine has enough of them to keep HBM busy, and add their sums through shared memory in a
-// fixed order.
+// share of the K chunks (256 values, 128 bytes of each row), which it copies into its own ring
+// of shared-memory stages with cp.async, whole lines at a time: the load pipe looks up one line
+// a clock, and fragments read from global memory directly cost it 8 lines per 256 bytes. Warps
+// of a CTA split K until the machine has enough of them to keep HBM busy, and add their sums
+// through shared memory in a fixed order. The rows of x stay in shared memory, already paired.
 #include <algorithm>
+#include <atomic>
 
 #include "matmul_internal.h"
 #include "qkv_common.cuh"
@@ -61,15 +64,32 @@ struct Codes<__half> {
   }
 };
 
-__device__ __forceinline__ uint2 ld_stream(const void* p) {
+__device__ __forceinline__ uint2 lds_v2(uint32_t at) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
   return v;
 }
-
-__device__ __forceinline__ uint4 ld_x(const void* p) { return __ldg((const uint4*)p); }
+__device__ __forceinline__ uint4 lds_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_v4(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+               : "memory");
+}
 
 // The expert and the first row of token chunk `id` (chunks of `per` rows, experts in order),
 // by a whole warp; false past the last chunk. Offsets are clamped into [0, R], and a
@@ -107,21 +127,39 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
   return false;
 }
 
-// MT token tiles of 8; GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same outputs
-template <typename T, int MT, bool GATED>
-__global__ void __launch_bounds__(kWarps * 32)
-    matmul_rows_kernel(const MatmulArgs a, int wk_count, int tiles) {
-  __shared__ float red[kWarps][MT * 4][32];
+constexpr int kStages = 4;                  // of one chunk, per warp
+constexpr int kCodeBytes = 16 * 128;        // 16 weight rows
+constexpr int kStageBytes = kCodeBytes + 2 * 16 * 8;  // and four scales and biases of each
+constexpr int kXBytes = 128 * 1024;         // most shared memory for rows of x
+
+struct RowsArgs {
+  MatmulArgs a;
+  int wk_count;  // warps that share K
+  int tiles;     // of 16 weight rows
+  int per;       // rows of x per CTA (at most 8 MT)
+};
+
+// MT: tiles of 8 rows of x. GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same
+// outputs. SB: how a row's four scales of a chunk are copied (8 bytes, 2 x 4, or one by one).
+template <typename T, int MT, bool GATED, int SB>
+__global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsArgs p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][kWarps][MT * 4][32];
   __shared__ int seg[3];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // what follows in the stream may be set up meanwhile; everything here may come from the
+  // kernel before, the weights too, so nothing is read before it is done
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const MatmulArgs& a = p.a;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  constexpr int PER = 8 * MT;
+  const int wk_count = p.wk_count;
 
   int expert = 0, row0, row1;
   if (a.offsets) {
     if (warp == 0) {
       int e = 0, r0 = 0, r1 = -1;
-      find_chunk(a.offsets, a.E, a.R, PER, blockIdx.y, lane, e, r0, r1);
+      find_chunk(a.offsets, a.E, a.R, p.per, blockIdx.y, lane, e, r0, r1);
       if (lane == 0) {
         seg[0] = e;
         seg[1] = r0;
@@ -129,199 +167,279 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
     }
     __syncthreads();
-    expert = seg[0];
-    row0 = seg[1];
-    row1 = seg[2];
+    expert = __shfl_sync(0xffffffffu, seg[0], 0);
+    row0 = __shfl_sync(0xffffffffu, seg[1], 0);
+    row1 = __shfl_sync(0xffffffffu, seg[2], 0);
     if (row1 < 0) return;
   } else {
-    row0 = blockIdx.y * PER;
-    row1 = min(row0 + PER, a.R);
+    row0 = blockIdx.y * p.per;
+    row1 = min(row0 + p.per, a.R);
   }
-
-  const int wk = warp % wk_count, wn = warp / wk_count;
-  const int tile = blockIdx.x * (kWarps / wk_count) + wn;
+  const int rows = row1 - row0;
+  const int wk = warp % wk_count, wn = warp / wk_count, wn_count = kWarps / wk_count;
   const int n_out = GATED ? a.N / 2 : a.N;
-  const int G = a.K / 64, chunks = (a.K + kChunk - 1) / kChunk;
-  // weight rows of this lane (clamped into the matrix; what is past it is not stored)
-  const int nA = GATED ? tile * 8 + g : tile * 16 + g;
-  const int nB = GATED ? nA : nA + 8;
-  const int last = n_out - 1;
-  const long long rA = (long long)expert * a.N + min(nA, last);
-  const long long rB = (long long)expert * a.N + min(nB, last) + (GATED ? n_out : 0);
-  const char* wA = (const char*)a.w + rA * (a.K / 2) + t * 8;
-  const char* wB = (const char*)a.w + rB * (a.K / 2) + t * 8;
-  const uint16_t* sA = (const uint16_t*)a.scales + rA * G;
-  const uint16_t* sB = (const uint16_t*)a.scales + rB * G;
-  const uint16_t* bA = (const uint16_t*)a.biases + rA * G;
-  const uint16_t* bB = (const uint16_t*)a.biases + rB * G;
+  const int G = a.K / 64, chunks = (a.K + kChunk - 1) / kChunk, pieces = a.K / 32;
+  const int units = (p.tiles + wn_count - 1) / wn_count;  // of wn_count tiles
+  const uint32_t xs = smem_u32(smem);
+  const uint32_t ring = xs + (uint32_t)rows * a.K * 2 + warp * kStages * kStageBytes;
 
-  // rows of x: token g of each tile
-  const char* xp[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = row0 + m * 8 + g;
-    int src = -1;
-    if (r < row1) src = a.rows ? a.rows[r] : r;
-    xp[m] = src >= 0 && src < a.x_rows
-                ? (const char*)a.x + ((long long)src * a.ldx + t * 16) * 2
-                : nullptr;
-  }
-
-  float acc[MT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
-
-  uint2 pa[4], pb[4];          // packed codes of the chunk: rows g and g + 8
-  uint32_t ps = 0, pbias = 0;  // (row g | row g+8 << 16) scale and bias of group t
-  auto load_w = [&](int c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool in = c < chunks && c * 4 + j < G;
-      pa[j] = in ? ld_stream(wA + (long long)c * 128 + j * 32) : make_uint2(0, 0);
-      pb[j] = in ? ld_stream(wB + (long long)c * 128 + j * 32) : make_uint2(0, 0);
-    }
-    ps = pbias = 0;
-    if (c < chunks && c * 4 + t < G) {
-      ps = sA[c * 4 + t] | (uint32_t)sB[c * 4 + t] << 16;
-      pbias = bA[c * 4 + t] | (uint32_t)bB[c * 4 + t] << 16;
-    }
+  // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
+  // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
+  auto weight_row = [&](int tile, int r) -> long long {
+    const int n = GATED ? min(tile * 8 + (r & 7), n_out - 1) + (r >> 3) * n_out
+                        : min(tile * 16 + r, n_out - 1);
+    return (long long)expert * a.N + n;
   };
-  auto load_x = [&](int gi, uint4 (&v)[MT][2]) {
+  int ld_unit = blockIdx.x, ld_c = wk, ld_slot = 0;
+  const char* src[4];   // this lane's 16 bytes of rows lane/8 + 4i
+  const char* ssrc;     // scales of row lane (biases of row lane - 16)
+  auto set_src = [&]() {
+    const int tile = min(ld_unit * wn_count + wn, p.tiles - 1);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const bool in = xp[m] && gi < G;
-      v[m][0] = in ? ld_x(xp[m] + (long long)gi * 128) : make_uint4(0, 0, 0, 0);
-      v[m][1] = in ? ld_x(xp[m] + (long long)gi * 128 + 16) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < 4; ++i)
+      src[i] = (const char*)a.w + weight_row(tile, (lane >> 3) + 4 * i) * (a.K / 2) + (lane & 7) * 16;
+    ssrc = (const char*)(lane < 16 ? a.scales : a.biases) + weight_row(tile, lane & 15) * G * 2;
   };
-
-  if (tile < tiles) {
-    uint4 xn[MT][2];
-    load_w(wk);
-    load_x(wk * 4, xn);
-    for (int c = wk; c < chunks; c += wk_count) {
-      uint2 ca[4], cb[4];
+  set_src();
+  auto load = [&]() {
+    if (ld_unit < units && ld_c < chunks) {
+      const uint32_t at = ring + ld_slot * kStageBytes;
+      if (ld_c * 8 + (lane & 7) < pieces) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ca[j] = pa[j];
-        cb[j] = pb[j];
+        for (int i = 0; i < 4; ++i) {
+          const int r = (lane >> 3) + 4 * i;  // (the swizzle keeps the fragment reads apart)
+          cp16(at + r * 128 + (((lane & 7) ^ (r & 3) << 1) << 4), src[i] + (long long)ld_c * 128);
+        }
       }
-      const uint32_t cs = ps, cbias = pbias;
-      load_w(c + wk_count);
+      const uint32_t to = at + kCodeBytes + lane * 8;
+      const char* from = ssrc + ld_c * 8;
+      if (SB == 2) {
+        cp_small<8>(to, from);
+      } else if (SB == 1) {
+        cp_small<4>(to, from);
+        if (ld_c * 4 + 2 < G) cp_small<4>(to + 4, from + 4);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (ld_c * 4 + j < G) {
+            const uint16_t v = __ldg((const uint16_t*)from + j);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 2 * j), "h"(v) : "memory");
+          }
+      }
+      ld_c += wk_count;
+      if (ld_c >= chunks) {
+        ld_c = wk;
+        ld_unit += gridDim.x;
+        set_src();
+      }
+    }
+    ld_slot = ld_slot + 1 == kStages ? 0 : ld_slot + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) load();
+
+  // ---- rows of x: 128 bytes per (group, row), the 32 bytes of lane t at 32 t, values paired
+  // as the codes are, the two halves of odd rows swapped (their reads then share no bank) -----
+  for (int i = threadIdx.x; i < rows * G * 4; i += kWarps * 32) {
+    const int m = i / (G * 4), q = i - m * (G * 4);  // q = group * 4 + t
+    const int r = row0 + m;
+    const int from = a.rows ? a.rows[r] : r;
+    uint4 u = make_uint4(0, 0, 0, 0), v = u;
+    if (from >= 0 && from < a.x_rows) {
+      const uint4* at = (const uint4*)((const char*)a.x + ((long long)from * a.ldx + q * 16) * 2);
+      u = __ldg(at);
+      v = __ldg(at + 1);
+    }
+    const uint32_t to = xs + ((q >> 2) * rows + m) * 128 + (q & 3) * 32;
+    sts_v4(to + (m & 1) * 16, make_uint4(prmt(u.x, u.z, 0x5410), prmt(u.x, u.z, 0x7632),
+                                         prmt(u.y, u.w, 0x5410), prmt(u.y, u.w, 0x7632)));
+    sts_v4(to + (~m & 1) * 16, make_uint4(prmt(v.x, v.z, 0x5410), prmt(v.x, v.z, 0x7632),
+                                          prmt(v.y, v.w, 0x5410), prmt(v.y, v.w, 0x7632)));
+  }
+  __syncthreads();
+
+  const uint32_t my_x = xs + g * 128 + t * 32;
+  const uint32_t code_at = g * 128 + (t & 1) * 8;
+  int slot = 0, buf = 0;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int tile = unit * wn_count + wn;
+    float acc[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
+
+    for (int c = wk; c < chunks; c += wk_count) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();
+      const uint32_t at = ring + slot * kStageBytes;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+      load();  // into the stage of the chunk before
+      // scales and biases of rows g and g + 8, four groups each
+      const uint2 sA = lds_v2(at + kCodeBytes + g * 8), sB = lds_v2(at + kCodeBytes + 64 + g * 8);
+      const uint2 bA = lds_v2(at + kCodeBytes + 128 + g * 8), bB = lds_v2(at + kCodeBytes + 192 + g * 8);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t xr[MT][8];
+        if (c * 4 + j >= G) break;
+        const uint32_t ca = at + code_at + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4);
+        const uint2 wa = lds_v2(ca), wb = lds_v2(ca + 1024);
+        uint4 xv[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          xv[m][0] = xv[m][1] = make_uint4(0, 0, 0, 0);
+          if (m * 8 + g < rows) {
+            const uint32_t xa = my_x + ((c * 4 + j) * rows + m * 8) * 128;
+            xv[m][0] = lds_v4(xa + (g & 1) * 16);
+            xv[m][1] = lds_v4(xa + (~g & 1) * 16);
+          }
+        }
+        float d[MT][4], sx[MT][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 v = xn[m][i];
-            xr[m][i * 4 + 0] = prmt(v.x, v.z, 0x5410);
-            xr[m][i * 4 + 1] = prmt(v.x, v.z, 0x7632);
-            xr[m][i * 4 + 2] = prmt(v.y, v.w, 0x5410);
-            xr[m][i * 4 + 3] = prmt(v.y, v.w, 0x7632);
-          }
-        load_x(j < 3 ? c * 4 + j + 1 : (c + wk_count) * 4, xn);
-        if (c * 4 + j < G) {
-          float d[MT][4], sx[MT][4];
+          for (int i = 0; i < 4; ++i) d[m][i] = sx[m][i] = 0.f;
+        const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes,
+                                  Codes<T>::kOnes};
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t u = i ? wa.y : wa.x, v = i ? wb.y : wb.x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[m][i] = sx[m][i] = 0.f;
-          const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes,
-                                    Codes<T>::kOnes};
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t f[4] = {and_or(u >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
+                                   and_or(v >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
+                                   and_or(u >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic),
+                                   and_or(v >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic)};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t u = i ? ca[j].y : ca[j].x, v = i ? cb[j].y : cb[j].x;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t f[4] = {and_or(u >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
-                                     and_or(v >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
-                                     and_or(u >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic),
-                                     and_or(v >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic)};
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                Codes<T>::mma(d[m], f, xr[m][i * 4 + h * 2], xr[m][i * 4 + h * 2 + 1]);
-                Codes<T>::mma(sx[m], ones, xr[m][i * 4 + h * 2], xr[m][i * 4 + h * 2 + 1]);
-              }
+            for (int m = 0; m < MT; ++m) {
+              const uint32_t b0 = h ? xv[m][i].z : xv[m][i].x, b1 = h ? xv[m][i].w : xv[m][i].y;
+              Codes<T>::mma(d[m], f, b0, b1);
+              Codes<T>::mma(sx[m], ones, b0, b1);
             }
           }
-          // scale and bias of group j live in lane j of the quad
-          const uint32_t s2 = __shfl_sync(0xffffffffu, cs, (lane & ~3) | j);
-          const uint32_t b2 = __shfl_sync(0xffffffffu, cbias, (lane & ~3) | j);
-          const float s0 = Elem<T>::bits_to_f32((uint16_t)s2), s1 = Elem<T>::bits_to_f32((uint16_t)(s2 >> 16));
-          const float b0 = Codes<T>::bias(s0, Elem<T>::bits_to_f32((uint16_t)b2));
-          const float b1 = Codes<T>::bias(s1, Elem<T>::bits_to_f32((uint16_t)(b2 >> 16)));
-          const float q0 = Codes<T>::scale(s0), q1 = Codes<T>::scale(s1);
+        }
+        const uint32_t s0 = j < 2 ? sA.x : sA.y, s1 = j < 2 ? sB.x : sB.y;
+        const uint32_t b0 = j < 2 ? bA.x : bA.y, b1 = j < 2 ? bB.x : bB.y;
+        const int sh = (j & 1) * 16;
+        const float f0 = Elem<T>::bits_to_f32((uint16_t)(s0 >> sh));
+        const float f1 = Elem<T>::bits_to_f32((uint16_t)(s1 >> sh));
+        const float o0 = Codes<T>::bias(f0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
+        const float o1 = Codes<T>::bias(f1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
+        const float q0 = Codes<T>::scale(f0), q1 = Codes<T>::scale(f1);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            acc[m][0] = fmaf(q0, d[m][0], fmaf(b0, sx[m][0], acc[m][0]));
-            acc[m][1] = fmaf(q0, d[m][1], fmaf(b0, sx[m][1], acc[m][1]));
-            acc[m][2] = fmaf(q1, d[m][2], fmaf(b1, sx[m][0], acc[m][2]));
-            acc[m][3] = fmaf(q1, d[m][3], fmaf(b1, sx[m][1], acc[m][3]));
-          }
+        for (int m = 0; m < MT; ++m) {
+          acc[m][0] = fmaf(q0, d[m][0], fmaf(o0, sx[m][0], acc[m][0]));
+          acc[m][1] = fmaf(q0, d[m][1], fmaf(o0, sx[m][1], acc[m][1]));
+          acc[m][2] = fmaf(q1, d[m][2], fmaf(o1, sx[m][0], acc[m][2]));
+          acc[m][3] = fmaf(q1, d[m][3], fmaf(o1, sx[m][1], acc[m][3]));
         }
       }
     }
-  }
 
-  if (wk_count > 1) {
-    if (wk) {
+    if (wk_count > 1) {
+      // (two buffers: the reader of this unit's passes the next unit's barrier before anyone
+      // writes here again)
+      if (wk) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[warp][m * 4 + i][lane] = acc[m][i];
-    }
-    __syncthreads();
-    if (wk) return;
-    for (int o = 1; o < wk_count; ++o)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] += red[warp + o][m * 4 + i][lane];
-  }
-  if (tile >= tiles) return;
-
-  T* out = (T*)a.out;
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = row0 + m * 8 + t * 2 + i;
-      if (r >= row1) continue;
-      T* o = out + (long long)r * n_out;
-      if (GATED) {
-        const float gate = acc[m][i], up = acc[m][i + 2];
-        if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
-      } else {
-        if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[m][i]);
-        if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[m][i + 2]);
+          for (int i = 0; i < 4; ++i) red[buf][warp][m * 4 + i][lane] = acc[m][i];
       }
+      named_bar_sync(1 + wn, wk_count * 32);
+      if (!wk) {
+        for (int o = 1; o < wk_count; ++o)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][i] += red[buf][warp + o][m * 4 + i][lane];
+      }
+      buf ^= 1;
     }
+    if (wk == 0 && tile < p.tiles) {
+      const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
+      T* out = (T*)a.out;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = m * 8 + t * 2 + i;
+          if (r >= rows) continue;
+          T* o = out + (long long)(row0 + r) * n_out;
+          if (GATED) {
+            const float gate = acc[m][i], up = acc[m][i + 2];
+            if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
+          } else {
+            if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[m][i]);
+            if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[m][i + 2]);
+          }
+        }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T, int MT, bool GATED, int SB>
+int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
+  static std::atomic<unsigned long long> ready{0};  // devices whose shared memory bound is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ECUDA;
+  if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(matmul_rows_kernel<T, MT, GATED, SB>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kXBytes + kWarps * kStages * kStageBytes) != cudaSuccess)
+      return QKV_ECUDA;
+    if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, matmul_rows_kernel<T, MT, GATED, SB>, p) == cudaSuccess
+             ? QKV_OK
+             : QKV_ECUDA;
+}
+
+template <typename T, int MT, bool GATED>
+int launch_rows_g(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
+  const int groups = p.a.K / 64;
+  const uintptr_t at = (uintptr_t)p.a.scales | (uintptr_t)p.a.biases;
+  if (groups % 4 == 0 && at % 8 == 0) return launch_rows_s<T, MT, GATED, 2>(p, grid, smem, st);
+  if (groups % 2 == 0 && at % 4 == 0) return launch_rows_s<T, MT, GATED, 1>(p, grid, smem, st);
+  return launch_rows_s<T, MT, GATED, 0>(p, grid, smem, st);
 }
 
 template <typename T, int MT>
 int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   const bool gated = a.act == QKV_ACT_SWIGLU;
   const int n_out = gated ? a.N / 2 : a.N;
-  const int tiles = gated ? (n_out + 7) / 8 : (n_out + 15) / 16;
-  const int per = 8 * MT;
-  long long segs = (a.R + per - 1) / per;
-  if (a.offsets) segs = std::min<long long>(a.R, (long long)std::min(a.E, a.R) + segs);
+  RowsArgs p;
+  p.a = a;
+  p.tiles = gated ? (n_out + 7) / 8 : (n_out + 15) / 16;
+  p.per = std::min(8 * MT, kXBytes / (a.K * 2));
+  if (p.per < 1) return QKV_EUNSUPPORTED;
+  long long segs = (a.R + p.per - 1) / p.per;
+  if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
   if (segs > 65535) return QKV_EUNSUPPORTED;
   const int chunks = (a.K + kChunk - 1) / kChunk;
+  const int sms = num_sms();
   // warps share K until the machine holds enough of them to keep HBM busy
-  int wk = 1;
-  while (wk < kWarps && wk * 2 <= chunks && (long long)tiles * segs * wk < 16ll * num_sms()) wk *= 2;
-  const int wn = kWarps / wk;
-  const dim3 grid((unsigned)((tiles + wn - 1) / wn), (unsigned)segs);
-  if (gated)
-    matmul_rows_kernel<T, MT, true><<<grid, kWarps * 32, 0, st>>>(a, wk, tiles);
-  else
-    matmul_rows_kernel<T, MT, false><<<grid, kWarps * 32, 0, st>>>(a, wk, tiles);
-  return QKV_OK;
+  p.wk_count = 1;
+  while (p.wk_count < kWarps && p.wk_count * 2 <= chunks &&
+         (long long)p.tiles * segs * p.wk_count < 16ll * sms)
+    p.wk_count *= 2;
+  const int units = (p.tiles + kWarps / p.wk_count - 1) / (kWarps / p.wk_count);
+  const size_t smem = (size_t)std::min(p.per, a.R) * a.K * 2 + kWarps * kStages * kStageBytes;
+  const int resident = sms * (smem > 110 * 1024 ? 1 : 2);
+  const long long wanted = (resident + segs - 1) / segs;
+  const dim3 grid((unsigned)std::min<long long>(units, a.offsets ? 2 * wanted : wanted), (unsigned)segs);
+  return gated ? launch_rows_g<T, MT, true>(p, grid, smem, st)
+               : launch_rows_g<T, MT, false>(p, grid, smem, st);
 }
 
 }  // namespace
