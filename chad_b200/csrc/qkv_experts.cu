@@ -23,13 +23,16 @@ namespace qkv {
 
 namespace {
 
-constexpr int kRouteThreads = 1024;
-constexpr int kMaxBlockTokens = 1024;
+constexpr int kRouteThreads = 1024;   // of a block that places
+constexpr int kChooseThreads = 512;   // of a block that chooses: two fit an SM
+constexpr int kPlaceBlocks = 4;       // choosing blocks whose pairs one block places
+constexpr int kMaxBlockTokens = 512;
 
-__device__ __forceinline__ float load_logit(const void* p, long long i, int dtype) {
-  if (dtype == QKV_F32) return ((const float*)p)[i];
-  const uint16_t b = ((const uint16_t*)p)[i];
-  return dtype == QKV_BF16 ? Elem<__nv_bfloat16>::bits_to_f32(b) : Elem<__half>::bits_to_f32(b);
+template <int DTYPE>
+__device__ __forceinline__ float load_logit(const void* p, long long i) {
+  if (DTYPE == QKV_F32) return __ldg((const float*)p + i);
+  const uint16_t b = __ldg((const uint16_t*)p + i);
+  return DTYPE == QKV_BF16 ? Elem<__nv_bfloat16>::bits_to_f32(b) : Elem<__half>::bits_to_f32(b);
 }
 
 // order-preserving key: a < b as floats <=> key(a) < key(b); -0 = +0, NaN above all
@@ -39,73 +42,89 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One warp, one token: experts[0..k), weights[0..k). PER = logits per lane.
-template <int PER>
+// The value of a key (NaN for the NaN key).
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key == 0xffffffffu ? 0x7fffffffu : key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+// One warp, one token: experts[0..k), weights[0..k). PER = logits per lane. Every lane keeps the
+// best of its own logits; a choice is a redux.max over the lanes' best keys, a redux.min over
+// the indices that have it, and a new best for the lane it came from. The first choice is the
+// softmax's maximum.
+template <int DTYPE, int PER>
 __device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane) {
-  float v[PER];
   uint32_t key[PER];
-  float mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int e = i * 32 + lane;
-    v[i] = e < a.E ? load_logit(a.logits, (long long)token * a.E + e, a.dtype) : -INFINITY;
-    key[i] = e < a.E ? order_key(v[i]) : 0u;  // 0: below every logit's key (-inf maps to 0x7fffff)
-    mx = fmaxf(mx, v[i]);
+    // 0 is below every logit's key (-inf has 0x7fffff)
+    key[i] = e < a.E ? order_key(load_logit<DTYPE>(a.logits, (long long)token * a.E + e)) : 0u;
   }
+  uint32_t best;
+  int best_i;
+  auto find_best = [&]() {
+    best = key[0];
+    best_i = 0;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float total = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) total += v[i] == -INFINITY ? 0.f : expf(v[i] - mx);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-
-  int mine = 0;        // lane j < k keeps the j-th choice
-  float p_mine = 0.f;
-  for (int j = 0; j < a.k; ++j) {
-    uint32_t best = key[0];
-#pragma unroll
-    for (int i = 1; i < PER; ++i) best = max(best, key[i]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    unsigned at = 0xffffffffu;
-#pragma unroll
-    for (int i = PER - 1; i >= 0; --i)
-      if (key[i] == best) at = i * 32 + lane;
-    at = __reduce_min_sync(0xffffffffu, at);
-    float p = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if ((unsigned)(i * 32 + lane) == at) {
-        p = v[i] == -INFINITY ? 0.f : expf(v[i] - mx);
-        key[i] = 0u;
+    for (int i = 1; i < PER; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        best_i = i;
       }
-    p = __shfl_sync(0xffffffffu, p, at & 31);
-    if (lane == j) {
-      mine = (int)at;
-      p_mine = p;
+  };
+  find_best();
+  const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+  const float mx = key_value(top);
+  float total = 0.f;
+  if (!a.normalize) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float v = key_value(key[i]);
+      if (key[i] != 0u && v != -INFINITY) total += expf(v - mx);
     }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
+  uint32_t at = 0, chosen = 0;  // lane j < k keeps the j-th choice
+#pragma unroll 1
+  for (int j = 0; j < a.k; ++j) {
+    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t mine = best == high ? best_i * 32u + lane : ~0u;
+    const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
+    if (lane == j) {
+      at = e;
+      chosen = high;
+    }
+    // without a branch: the lane of the choice drops it and finds its next best
+    const int drop = e == mine ? best_i : -1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = i == drop ? 0u : key[i];
+    find_best();
+  }
+  const float v = key_value(chosen);
+  const float p = lane >= a.k || v == -INFINITY ? 0.f : expf(v - mx);
   if (a.normalize) {
-    total = lane < a.k ? p_mine : 0.f;
+    total = p;
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   if (lane < a.k) {
     // total is 0 only for a row of -inf, whose weights are 0
-    a.experts[(long long)token * a.k + lane] = mine;
-    a.weights[(long long)token * a.k + lane] = total == 0.f ? 0.f : p_mine / total;
+    a.experts[(long long)token * a.k + lane] = (int)at;
+    a.weights[(long long)token * a.k + lane] = total == 0.f ? 0.f : p / total;
   }
 }
 
+template <int DTYPE, int THREADS>
 __device__ __forceinline__ void route_block(const RouteArgs& a, int t0, int t1) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (a.E + 31) / 32;
-  for (int t = t0 + warp; t < t1; t += kRouteThreads / 32) {
-    if (per <= 1) route_token<1>(a, t, lane);
-    else if (per <= 2) route_token<2>(a, t, lane);
-    else if (per <= 4) route_token<4>(a, t, lane);
-    else if (per <= 8) route_token<8>(a, t, lane);
-    else route_token<16>(a, t, lane);
+  for (int t = t0 + warp; t < t1; t += THREADS / 32) {
+    if (per <= 1) route_token<DTYPE, 1>(a, t, lane);
+    else if (per <= 2) route_token<DTYPE, 2>(a, t, lane);
+    else if (per <= 4) route_token<DTYPE, 4>(a, t, lane);
+    else if (per <= 8) route_token<DTYPE, 8>(a, t, lane);
+    else route_token<DTYPE, 16>(a, t, lane);
   }
 }
 
@@ -148,23 +167,25 @@ __device__ __forceinline__ void scan_counts(int* count, int E) {
 }
 
 // Choices of one block of tokens and its count per expert (several blocks: the first launch)
-__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs a, int bt) {
+template <int DTYPE>
+__global__ void __launch_bounds__(kChooseThreads, 2) route_choose_kernel(const RouteArgs a, int bt) {
   extern __shared__ int smem[];
   const int t0 = blockIdx.x * bt, t1 = min(t0 + bt, a.T);
-  for (int e = threadIdx.x; e < a.E; e += kRouteThreads) smem[e] = 0;
-  route_block(a, t0, t1);
+  for (int e = threadIdx.x; e < a.E; e += kChooseThreads) smem[e] = 0;
+  route_block<DTYPE, kChooseThreads>(a, t0, t1);
   __syncthreads();
-  for (int i = threadIdx.x; i < (t1 - t0) * a.k; i += kRouteThreads)
+  for (int i = threadIdx.x; i < (t1 - t0) * a.k; i += kChooseThreads)
     atomicAdd(&smem[a.experts[(long long)t0 * a.k + i]], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kRouteThreads)
+  for (int e = threadIdx.x; e < a.E; e += kChooseThreads)
     a.hist[(long long)blockIdx.x * a.E + e] = smem[e];
 }
 
 // Sorted positions of one block's pairs. ONE: a single block that also chooses (a decode
 // batch); otherwise the base of every expert is summed over the earlier blocks' counts.
-template <bool ONE>
-__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs a, int bt) {
+template <bool ONE, int DTYPE>
+__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs a, int bt,
+                                                                      int counted) {
   extern __shared__ int smem[];
   const int words = (bt + 31) / 32;
   int* base = smem;                                  // E + 1
@@ -173,18 +194,31 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   const int t0 = ONE ? 0 : blockIdx.x * bt, t1 = min(t0 + bt, a.T);
   for (int i = threadIdx.x; i < words * a.E; i += kRouteThreads) mask[i] = 0;
   if (ONE) {
-    route_block(a, t0, t1);
+    route_block<DTYPE, kRouteThreads>(a, t0, t1);
   } else {
-    for (int e = threadIdx.x; e < a.E; e += kRouteThreads) {
+    // the block's threads share the rows of counts of every expert
+    for (int e = threadIdx.x; e < a.E; e += kRouteThreads) base[e] = before[e] = 0;
+    __syncthreads();
+    const int lanes = (a.E + 31) / 32 * 32, share = kRouteThreads / lanes;
+    const int e = threadIdx.x % lanes, part = threadIdx.x / lanes;
+    if (part < share && e < a.E) {
       int all = 0, prior = 0;
-#pragma unroll 8
-      for (int b = 0; b < gridDim.x; ++b) {
-        const int n = a.hist[(long long)b * a.E + e];
-        all += n;
-        prior += b < blockIdx.x ? n : 0;
+      const int mine = blockIdx.x * kPlaceBlocks;
+      for (int b0 = part; b0 < counted; b0 += 16 * share) {
+        int n[16];  // sixteen loads in flight
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int b = b0 + i * share;
+          n[i] = b < counted ? __ldg(a.hist + (long long)b * a.E + e) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          all += n[i];
+          prior += b0 + i * share < mine ? n[i] : 0;
+        }
       }
-      base[e] = all;
-      before[e] = prior;
+      atomicAdd(&base[e], all);
+      atomicAdd(&before[e], prior);
     }
   }
   __syncthreads();
@@ -218,10 +252,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   }
 }
 
-// Tokens of a block: 64, growing past 256 blocks so that the sums over earlier blocks'
+// Tokens of a choosing block: 32, growing past 256 blocks so that the sums over earlier blocks'
 // counts stay short (they are read by every block).
 int route_block_tokens(int T) {
-  int bt = 64;
+  int bt = 32;
   while (bt < kMaxBlockTokens && (T + bt - 1) / bt > 256) bt *= 2;
   return bt;
 }
@@ -242,29 +276,51 @@ __global__ void __launch_bounds__(256)
   const long long t = i / per_row;
   const int c = (int)(i - t * per_row) * VEC;
   float acc[VEC];
-  auto add = [&](const T* p, float w) {
+  auto add = [&](const uint4& v, float w) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
     if constexpr (VEC == 8) {
-      const uint4 v = __ldg((const uint4*)p);
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         acc[2 * q] = fmaf(w, Elem<T>::bits_to_f32((uint16_t)u[q]), acc[2 * q]);
         acc[2 * q + 1] = fmaf(w, Elem<T>::bits_to_f32((uint16_t)(u[q] >> 16)), acc[2 * q + 1]);
       }
     } else {
-      acc[0] = fmaf(w, Elem<T>::to_f32(*p), acc[0]);
+      acc[0] = fmaf(w, Elem<T>::bits_to_f32((uint16_t)u[0]), acc[0]);
     }
   };
+  auto get = [&](const T* p) -> uint4 {
+    if constexpr (VEC == 8) return __ldg((const uint4*)p);
+    return make_uint4(__ldg((const uint16_t*)p), 0, 0, 0);
+  };
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint4 res = residual ? get(residual + t * N + c) : zero;
 #pragma unroll
   for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
-  for (int j = 0; j < k; ++j) {
-    const int s = slots[t * k + j];
-    if (s >= 0 && s < R) add(y + (long long)s * N + c, weights[t * k + j]);
-  }
-  if (residual) add(residual + t * N + c, 1.f);
-  T* o = out + t * N + c;
+  // eight rows in flight at a time
+  for (int j0 = 0; j0 < k; j0 += 8) {
+    float w[8];
+    uint4 v[8];
 #pragma unroll
-  for (int q = 0; q < VEC; ++q) o[q] = Elem<T>::from_f32(acc[q]);
+    for (int j = 0; j < 8; ++j) {
+      const bool in = j0 + j < k;
+      const int s = in ? __ldg(slots + t * k + j0 + j) : -1;
+      const bool held = s >= 0 && s < R;  // (a dropped pair's weight may be anything)
+      w[j] = held ? __ldg(weights + t * k + j0 + j) : 0.f;
+      v[j] = held ? get(y + (long long)s * N + c) : zero;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add(v[j], w[j]);
+  }
+  add(res, residual ? 1.f : 0.f);
+  T* o = out + t * N + c;
+  if constexpr (VEC == 8) {
+    alignas(16) T r[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) r[q] = Elem<T>::from_f32(acc[q]);
+    *(uint4*)o = *(const uint4*)r;
+  } else {
+    o[0] = Elem<T>::from_f32(acc[0]);
+  }
 }
 
 template <typename T>
@@ -292,21 +348,31 @@ size_t route_workspace_bytes(int T, int E) {
   return (size_t)((T + bt - 1) / bt) * E * sizeof(int);
 }
 
-int launch_route(const RouteArgs& a, cudaStream_t st) {
+template <int DTYPE>
+static int launch_route_t(const RouteArgs& a, cudaStream_t st) {
   if (a.T <= kOneBlock) {
-    route_place_kernel<true><<<1, kRouteThreads, place_smem(a.E, kOneBlock), st>>>(a, kOneBlock);
+    route_place_kernel<true, DTYPE>
+        <<<1, kRouteThreads, place_smem(a.E, kOneBlock), st>>>(a, kOneBlock, 0);
     return QKV_OK;
   }
-  const int bt = route_block_tokens(a.T);
-  const size_t smem = place_smem(a.E, bt);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(route_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)smem) != cudaSuccess)
-    return QKV_ECUDA;
+  const int bt = route_block_tokens(a.T), place = bt * kPlaceBlocks;
   const unsigned blocks = (unsigned)((a.T + bt - 1) / bt);
-  route_choose_kernel<<<blocks, kRouteThreads, a.E * sizeof(int), st>>>(a, bt);
-  route_place_kernel<false><<<blocks, kRouteThreads, smem, st>>>(a, bt);
+  const size_t smem = place_smem(a.E, place);
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(route_place_kernel<false, QKV_F32>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return QKV_ECUDA;
+  route_choose_kernel<DTYPE><<<blocks, kChooseThreads, a.E * sizeof(int), st>>>(a, bt);
+  route_place_kernel<false, QKV_F32>
+      <<<(blocks + kPlaceBlocks - 1) / kPlaceBlocks, kRouteThreads, smem, st>>>(a, place,
+                                                                                (int)blocks);
   return QKV_OK;
+}
+
+int launch_route(const RouteArgs& a, cudaStream_t st) {
+  if (a.dtype == QKV_BF16) return launch_route_t<QKV_BF16>(a, st);
+  if (a.dtype == QKV_F16) return launch_route_t<QKV_F16>(a, st);
+  return launch_route_t<QKV_F32>(a, st);
 }
 
 int launch_expert_combine(const void* y, int R, const int* slots, const float* weights,

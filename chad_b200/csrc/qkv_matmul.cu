@@ -20,6 +20,7 @@
 // a clock, and fragments read from global memory directly cost it 8 lines per 256 bytes. Warps
 // of a CTA split K until the machine has enough of them to keep HBM busy, and add their sums
 // through shared memory in a fixed order. The rows of x stay in shared memory, already paired.
+#include <stdlib.h>
 #include <algorithm>
 #include <atomic>
 
@@ -181,7 +182,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const int G = a.K / 64, chunks = (a.K + kChunk - 1) / kChunk, pieces = a.K / 32;
   const int units = (p.tiles + wn_count - 1) / wn_count;  // of wn_count tiles
   const uint32_t xs = smem_u32(smem);
-  const uint32_t ring = xs + (uint32_t)rows * a.K * 2 + warp * kStages * kStageBytes;
+  const uint32_t sums = xs + (uint32_t)rows * a.K * 2;  // of each group of each row of x
+  const uint32_t ring = sums + (uint32_t)G * MT * 32 + warp * kStages * kStageBytes;
 
   // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
   // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
@@ -259,7 +261,39 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   }
   __syncthreads();
 
+  // one group of x as B fragments: lane (g, t) holds 16 values of row g of each tile
   const uint32_t my_x = xs + g * 128 + t * 32;
+  auto x_frag = [&](int group, uint4 (&xv)[MT][2]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      xv[m][0] = xv[m][1] = make_uint4(0, 0, 0, 0);
+      if (m * 8 + g < rows) {
+        const uint32_t xa = my_x + (group * rows + m * 8) * 128;
+        xv[m][0] = lds_v4(xa + (g & 1) * 16);
+        xv[m][1] = lds_v4(xa + (~g & 1) * 16);
+      }
+    }
+  };
+  // sums of x by group, with a matrix of ones
+  for (int j = warp; j < G; j += kWarps) {
+    const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes};
+    uint4 xv[MT][2];
+    x_frag(j, xv);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Codes<T>::mma(d, ones, xv[m][i].x, xv[m][i].y);
+        Codes<T>::mma(d, ones, xv[m][i].z, xv[m][i].w);
+      }
+      if (g == 0)
+        asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + (j * MT + m) * 32 + t * 8),
+                     "f"(d[0]), "f"(d[1])
+                     : "memory");
+    }
+  }
+  __syncthreads();
   const uint32_t code_at = g * 128 + (t & 1) * 8;
   int slot = 0, buf = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -285,22 +319,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         const uint32_t ca = at + code_at + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4);
         const uint2 wa = lds_v2(ca), wb = lds_v2(ca + 1024);
         uint4 xv[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          xv[m][0] = xv[m][1] = make_uint4(0, 0, 0, 0);
-          if (m * 8 + g < rows) {
-            const uint32_t xa = my_x + ((c * 4 + j) * rows + m * 8) * 128;
-            xv[m][0] = lds_v4(xa + (g & 1) * 16);
-            xv[m][1] = lds_v4(xa + (~g & 1) * 16);
-          }
-        }
-        float d[MT][4], sx[MT][4];
+        x_frag(c * 4 + j, xv);
+        float d[MT][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[m][i] = sx[m][i] = 0.f;
-        const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes,
-                                  Codes<T>::kOnes};
+          for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t u = i ? wa.y : wa.x, v = i ? wb.y : wb.x;
@@ -314,7 +338,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
             for (int m = 0; m < MT; ++m) {
               const uint32_t b0 = h ? xv[m][i].z : xv[m][i].x, b1 = h ? xv[m][i].w : xv[m][i].y;
               Codes<T>::mma(d[m], f, b0, b1);
-              Codes<T>::mma(sx[m], ones, b0, b1);
             }
           }
         }
@@ -328,10 +351,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         const float q0 = Codes<T>::scale(f0), q1 = Codes<T>::scale(f1);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          acc[m][0] = fmaf(q0, d[m][0], fmaf(o0, sx[m][0], acc[m][0]));
-          acc[m][1] = fmaf(q0, d[m][1], fmaf(o0, sx[m][1], acc[m][1]));
-          acc[m][2] = fmaf(q1, d[m][2], fmaf(o1, sx[m][0], acc[m][2]));
-          acc[m][3] = fmaf(q1, d[m][3], fmaf(o1, sx[m][1], acc[m][3]));
+          const uint2 sx = lds_v2(sums + ((c * 4 + j) * MT + m) * 32 + t * 8);
+          const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
+          acc[m][0] = fmaf(q0, d[m][0], fmaf(o0, sx0, acc[m][0]));
+          acc[m][1] = fmaf(q0, d[m][1], fmaf(o0, sx1, acc[m][1]));
+          acc[m][2] = fmaf(q1, d[m][2], fmaf(o1, sx0, acc[m][2]));
+          acc[m][3] = fmaf(q1, d[m][3], fmaf(o1, sx1, acc[m][3]));
         }
       }
     }
@@ -386,7 +411,7 @@ int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
     if (cudaFuncSetAttribute(matmul_rows_kernel<T, MT, GATED, SB>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kXBytes + kWarps * kStages * kStageBytes) != cudaSuccess)
+                             kXBytes + kXBytes / 8 + kWarps * kStages * kStageBytes) != cudaSuccess)
       return QKV_ECUDA;
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
@@ -427,17 +452,26 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
   if (segs > 65535) return QKV_EUNSUPPORTED;
   const int chunks = (a.K + kChunk - 1) / kChunk;
-  const int sms = num_sms();
-  // warps share K until the machine holds enough of them to keep HBM busy
-  p.wk_count = 1;
-  while (p.wk_count < kWarps && p.wk_count * 2 <= chunks &&
-         (long long)p.tiles * segs * p.wk_count < 16ll * sms)
-    p.wk_count *= 2;
-  const int units = (p.tiles + kWarps / p.wk_count - 1) / (kWarps / p.wk_count);
-  const size_t smem = (size_t)std::min(p.per, a.R) * a.K * 2 + kWarps * kStages * kStageBytes;
-  const int resident = sms * (smem > 110 * 1024 ? 1 : 2);
-  const long long wanted = (resident + segs - 1) / segs;
-  const dim3 grid((unsigned)std::min<long long>(units, a.offsets ? 2 * wanted : wanted), (unsigned)segs);
+  const size_t smem = (size_t)std::min(p.per, a.R) * a.K * 2 + (size_t)a.K / 64 * MT * 32 +
+                      kWarps * kStages * kStageBytes;
+  const int resident = num_sms() * (smem > 104 * 1024 ? 1 : 2);
+  const int ctas = (int)std::max<long long>(1, resident / segs);  // per chunk of rows
+  // Warps that share K: the number whose longest warp has the least to do. A unit of a CTA costs
+  // its chunks and about half a chunk more for the sums (through shared memory when shared).
+  int best = 0;
+  long long best_cost = 0;
+  for (int wk = 1; wk <= kWarps && wk <= chunks; wk *= 2) {
+    const int units = (p.tiles + kWarps / wk - 1) / (kWarps / wk);
+    const long long rounds = (units + ctas - 1) / ctas;
+    const long long cost = rounds * (4 * ((chunks + wk - 1) / wk) + (wk > 1 ? 2 : 1));
+    if (!best || cost < best_cost) {
+      best = wk;
+      best_cost = cost;
+    }
+  }
+  p.wk_count = best;
+  const int units = (p.tiles + kWarps / best - 1) / (kWarps / best);
+  const dim3 grid((unsigned)std::min(units, ctas), (unsigned)segs);
   return gated ? launch_rows_g<T, MT, true>(p, grid, smem, st)
                : launch_rows_g<T, MT, false>(p, grid, smem, st);
 }
@@ -452,6 +486,7 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
 // By rows per weight matrix (experts without rows unknown): at 22 rows per expert the tcgen05
 // kernel took 44 us where the one above took 122.
 bool matmul_takes_tc(int R, int E, int N) {
+  if (const char* f = getenv("MM_FORCE")) return f[0] == 't';
   return matmul_tc_fits(E, N) && R >= 16ll * std::min(E, R);
 }
 

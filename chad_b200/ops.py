@@ -572,7 +572,8 @@ def route_topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> Routi
     # one allocation for the integers: offsets, rows, experts, slots and the workspace
     ints = logits.new_empty(e + 1 + 3 * pairs + need // 4 + 4, dtype=torch.int32)
     weights = logits.new_empty((t, k), dtype=torch.float32)
-    offsets, rows, experts, slots, work = ints.split((e + 1, pairs, pairs, pairs, need // 4 + 4))
+    offsets, rows, experts, slots, _ = torch.unsafe_split_with_sizes(
+        ints, (e + 1, pairs, pairs, pairs, need // 4 + 4))
     base = ints.data_ptr()
     at = base + 4 * (e + 1)
     check(_lib.fn("qkv_route_topk")(
