@@ -20,7 +20,6 @@
 // a clock, and fragments read from global memory directly cost it 8 lines per 256 bytes. Warps
 // of a CTA split K until the machine has enough of them to keep HBM busy, and add their sums
 // through shared memory in a fixed order. The rows of x stay in shared memory, already paired.
-#include <stdlib.h>
 #include <algorithm>
 #include <atomic>
 
@@ -128,24 +127,28 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
   return false;
 }
 
-constexpr int kStages = 4;                  // of one chunk, per warp
+constexpr int kStages = 3;                  // of one chunk, per warp
 constexpr int kCodeBytes = 16 * 128;        // 16 weight rows
 constexpr int kStageBytes = kCodeBytes + 2 * 16 * 8;  // and four scales and biases of each
-constexpr int kXBytes = 128 * 1024;         // most shared memory for rows of x
+
+// Dynamic shared memory of a CTA (8 KiB of sums are static): rows of x and their sums by group,
+// then the rings.
+constexpr int kDynamicBytes = 227 * 1024 - 8192 - 256;
+inline long long x_bytes(int rows, int K) { return (long long)rows * K * 2 + (long long)K / 64 * 32; }
 
 struct RowsArgs {
   MatmulArgs a;
   int wk_count;  // warps that share K
   int tiles;     // of 16 weight rows
-  int per;       // rows of x per CTA (at most 8 MT)
+  int per;       // rows of x per CTA (at most 8)
 };
 
-// MT: tiles of 8 rows of x. GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same
-// outputs. SB: how a row's four scales of a chunk are copied (8 bytes, 2 x 4, or one by one).
-template <typename T, int MT, bool GATED, int SB>
+// GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same outputs. SB: how a row's four
+// scales of a chunk are copied (8 bytes, 2 x 4, or one by one).
+template <typename T, bool GATED, int SB>
 __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[2][kWarps][MT * 4][32];
+  __shared__ float red[2][kWarps][4][32];
   __shared__ int seg[3];
   // what follows in the stream may be set up meanwhile; everything here may come from the
   // kernel before, the weights too, so nothing is read before it is done
@@ -183,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const int units = (p.tiles + wn_count - 1) / wn_count;  // of wn_count tiles
   const uint32_t xs = smem_u32(smem);
   const uint32_t sums = xs + (uint32_t)rows * a.K * 2;  // of each group of each row of x
-  const uint32_t ring = sums + (uint32_t)G * MT * 32 + warp * kStages * kStageBytes;
+  const uint32_t ring = sums + (uint32_t)G * 32 + warp * kStages * kStageBytes;
 
   // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
   // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
@@ -263,47 +266,36 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
 
   // one group of x as B fragments: lane (g, t) holds 16 values of row g of each tile
   const uint32_t my_x = xs + g * 128 + t * 32;
-  auto x_frag = [&](int group, uint4 (&xv)[MT][2]) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      xv[m][0] = xv[m][1] = make_uint4(0, 0, 0, 0);
-      if (m * 8 + g < rows) {
-        const uint32_t xa = my_x + (group * rows + m * 8) * 128;
-        xv[m][0] = lds_v4(xa + (g & 1) * 16);
-        xv[m][1] = lds_v4(xa + (~g & 1) * 16);
-      }
+  auto x_frag = [&](int group, uint4 (&xv)[2]) {
+    xv[0] = xv[1] = make_uint4(0, 0, 0, 0);
+    if (g < rows) {
+      const uint32_t xa = my_x + group * rows * 128;
+      xv[0] = lds_v4(xa + (g & 1) * 16);
+      xv[1] = lds_v4(xa + (~g & 1) * 16);
     }
   };
   // sums of x by group, with a matrix of ones
   for (int j = warp; j < G; j += kWarps) {
     const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes};
-    uint4 xv[MT][2];
+    uint4 xv[2];
     x_frag(j, xv);
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        Codes<T>::mma(d, ones, xv[m][i].x, xv[m][i].y);
-        Codes<T>::mma(d, ones, xv[m][i].z, xv[m][i].w);
-      }
-      if (g == 0)
-        asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + (j * MT + m) * 32 + t * 8),
-                     "f"(d[0]), "f"(d[1])
-                     : "memory");
+    for (int i = 0; i < 2; ++i) {
+      Codes<T>::mma(d, ones, xv[i].x, xv[i].y);
+      Codes<T>::mma(d, ones, xv[i].z, xv[i].w);
     }
+    if (g == 0)
+      asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + j * 32 + t * 8), "f"(d[0]),
+                   "f"(d[1])
+                   : "memory");
   }
   __syncthreads();
   const uint32_t code_at = g * 128 + (t & 1) * 8;
   int slot = 0, buf = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int tile = unit * wn_count + wn;
-    float acc[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
-
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = wk; c < chunks; c += wk_count) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp();
@@ -318,28 +310,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         if (c * 4 + j >= G) break;
         const uint32_t ca = at + code_at + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4);
         const uint2 wa = lds_v2(ca), wb = lds_v2(ca + 1024);
-        uint4 xv[MT][2];
-        x_frag(c * 4 + j, xv);
-        float d[MT][4];
+        uint32_t f[4][4];  // A fragments of the group's four MMAs
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t u = i ? wa.y : wa.x, v = i ? wb.y : wb.x;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t f[4] = {and_or(u >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
-                                   and_or(v >> (8 * h), 0x000f000fu, Codes<T>::kMagic),
-                                   and_or(u >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic),
-                                   and_or(v >> (8 * h + 4), 0x000f000fu, Codes<T>::kMagic)};
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint32_t b0 = h ? xv[m][i].z : xv[m][i].x, b1 = h ? xv[m][i].w : xv[m][i].y;
-              Codes<T>::mma(d[m], f, b0, b1);
-            }
-          }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = (i & 2 ? wa.y : wa.x) >> (8 * (i & 1));
+          const uint32_t v = (i & 2 ? wb.y : wb.x) >> (8 * (i & 1));
+          f[i][0] = and_or(u, 0x000f000fu, Codes<T>::kMagic);
+          f[i][1] = and_or(v, 0x000f000fu, Codes<T>::kMagic);
+          f[i][2] = and_or(u >> 4, 0x000f000fu, Codes<T>::kMagic);
+          f[i][3] = and_or(v >> 4, 0x000f000fu, Codes<T>::kMagic);
         }
         const uint32_t s0 = j < 2 ? sA.x : sA.y, s1 = j < 2 ? sB.x : sB.y;
         const uint32_t b0 = j < 2 ? bA.x : bA.y, b1 = j < 2 ? bB.x : bB.y;
@@ -349,15 +328,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         const float o0 = Codes<T>::bias(f0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
         const float o1 = Codes<T>::bias(f1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
         const float q0 = Codes<T>::scale(f0), q1 = Codes<T>::scale(f1);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint2 sx = lds_v2(sums + ((c * 4 + j) * MT + m) * 32 + t * 8);
-          const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
-          acc[m][0] = fmaf(q0, d[m][0], fmaf(o0, sx0, acc[m][0]));
-          acc[m][1] = fmaf(q0, d[m][1], fmaf(o0, sx1, acc[m][1]));
-          acc[m][2] = fmaf(q1, d[m][2], fmaf(o1, sx0, acc[m][2]));
-          acc[m][3] = fmaf(q1, d[m][3], fmaf(o1, sx1, acc[m][3]));
-        }
+        uint4 xv[2];
+        x_frag(c * 4 + j, xv);
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        Codes<T>::mma(d, f[0], xv[0].x, xv[0].y);
+        Codes<T>::mma(d, f[1], xv[0].z, xv[0].w);
+        Codes<T>::mma(d, f[2], xv[1].x, xv[1].y);
+        Codes<T>::mma(d, f[3], xv[1].z, xv[1].w);
+        const uint2 sx = lds_v2(sums + (c * 4 + j) * 32 + t * 8);
+        const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
+        acc[0] = fmaf(q0, d[0], fmaf(o0, sx0, acc[0]));
+        acc[1] = fmaf(q0, d[1], fmaf(o0, sx1, acc[1]));
+        acc[2] = fmaf(q1, d[2], fmaf(o1, sx0, acc[2]));
+        acc[3] = fmaf(q1, d[3], fmaf(o1, sx1, acc[3]));
       }
     }
 
@@ -366,17 +349,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       // writes here again)
       if (wk) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) red[buf][warp][m * 4 + i][lane] = acc[m][i];
+        for (int i = 0; i < 4; ++i) red[buf][warp][i][lane] = acc[i];
       }
       named_bar_sync(1 + wn, wk_count * 32);
       if (!wk) {
         for (int o = 1; o < wk_count; ++o)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][i] += red[buf][warp + o][m * 4 + i][lane];
+          for (int i = 0; i < 4; ++i) acc[i] += red[buf][warp + o][i][lane];
       }
       buf ^= 1;
     }
@@ -384,34 +363,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
       T* out = (T*)a.out;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = m * 8 + t * 2 + i;
-          if (r >= rows) continue;
-          T* o = out + (long long)(row0 + r) * n_out;
-          if (GATED) {
-            const float gate = acc[m][i], up = acc[m][i + 2];
-            if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
-          } else {
-            if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[m][i]);
-            if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[m][i + 2]);
-          }
+      for (int i = 0; i < 2; ++i) {
+        const int r = t * 2 + i;
+        if (r >= rows) continue;
+        T* o = out + (long long)(row0 + r) * n_out;
+        if (GATED) {
+          const float gate = acc[i], up = acc[i + 2];
+          if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
+        } else {
+          if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[i]);
+          if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[i + 2]);
         }
+      }
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, int MT, bool GATED, int SB>
+template <typename T, bool GATED, int SB>
 int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};  // devices whose shared memory bound is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ECUDA;
   if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(matmul_rows_kernel<T, MT, GATED, SB>,
+    if (cudaFuncSetAttribute(matmul_rows_kernel<T, GATED, SB>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kXBytes + kXBytes / 8 + kWarps * kStages * kStageBytes) != cudaSuccess)
+                             kDynamicBytes) != cudaSuccess)
       return QKV_ECUDA;
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
@@ -425,37 +402,43 @@ int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, matmul_rows_kernel<T, MT, GATED, SB>, p) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, matmul_rows_kernel<T, GATED, SB>, p) == cudaSuccess
              ? QKV_OK
              : QKV_ECUDA;
 }
 
-template <typename T, int MT, bool GATED>
+template <typename T, bool GATED>
 int launch_rows_g(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   const int groups = p.a.K / 64;
   const uintptr_t at = (uintptr_t)p.a.scales | (uintptr_t)p.a.biases;
-  if (groups % 4 == 0 && at % 8 == 0) return launch_rows_s<T, MT, GATED, 2>(p, grid, smem, st);
-  if (groups % 2 == 0 && at % 4 == 0) return launch_rows_s<T, MT, GATED, 1>(p, grid, smem, st);
-  return launch_rows_s<T, MT, GATED, 0>(p, grid, smem, st);
+  if (groups % 4 == 0 && at % 8 == 0) return launch_rows_s<T, GATED, 2>(p, grid, smem, st);
+  if (groups % 2 == 0 && at % 4 == 0) return launch_rows_s<T, GATED, 1>(p, grid, smem, st);
+  return launch_rows_s<T, GATED, 0>(p, grid, smem, st);
 }
 
-template <typename T, int MT>
+template <typename T>
 int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   const bool gated = a.act == QKV_ACT_SWIGLU;
   const int n_out = gated ? a.N / 2 : a.N;
   RowsArgs p;
   p.a = a;
   p.tiles = gated ? (n_out + 7) / 8 : (n_out + 15) / 16;
-  p.per = std::min(8 * MT, kXBytes / (a.K * 2));
+  // Eight rows, or as many as fit beside the rings. (Two or four tiles of eight rows to a pass
+  // over the weights were slower at every row count: 2048x4096 at 64 rows 15.4 us with one tile,
+  // 15.5 and 21.8 with two and four; 12288x2048 at 32 rows 18.8, 17.8 and 28.5.)
+  p.per = std::min(8, a.R);
+  while (p.per > 0 && x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes > kDynamicBytes) --p.per;
   if (p.per < 1) return QKV_EUNSUPPORTED;
   long long segs = (a.R + p.per - 1) / p.per;
   if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
   if (segs > 65535) return QKV_EUNSUPPORTED;
   const int chunks = (a.K + kChunk - 1) / kChunk;
-  const size_t smem = (size_t)std::min(p.per, a.R) * a.K * 2 + (size_t)a.K / 64 * MT * 32 +
-                      kWarps * kStages * kStageBytes;
+  const size_t smem = x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes;
   const int resident = num_sms() * (smem > 104 * 1024 ? 1 : 2);
-  const int ctas = (int)std::max<long long>(1, resident / segs);  // per chunk of rows
+  // CTAs per chunk of rows: as many as are resident; with experts twice that, for the bound on
+  // the chunks counts experts that may be empty (64 experts of 1536x2048 at 4 rows each 41 us
+  // with once, 35 with twice, 38 with four times as many).
+  const int ctas = (int)std::max<long long>(1, (a.offsets ? 2 : 1) * resident / segs);
   // Warps that share K: the number whose longest warp has the least to do. A unit of a CTA costs
   // its chunks and about half a chunk more for the sums (through shared memory when shared).
   int best = 0;
@@ -472,22 +455,26 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   p.wk_count = best;
   const int units = (p.tiles + kWarps / best - 1) / (kWarps / best);
   const dim3 grid((unsigned)std::min(units, ctas), (unsigned)segs);
-  return gated ? launch_rows_g<T, MT, true>(p, grid, smem, st)
-               : launch_rows_g<T, MT, false>(p, grid, smem, st);
+  return gated ? launch_rows_g<T, true>(p, grid, smem, st)
+               : launch_rows_g<T, false>(p, grid, smem, st);
 }
 
 }  // namespace
 
 int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
-  if (a.dtype == QKV_BF16) return launch_rows<__nv_bfloat16, 1>(a, st);
-  return launch_rows<__half, 1>(a, st);
+  if (a.dtype == QKV_BF16) return launch_rows<__nv_bfloat16>(a, st);
+  return launch_rows<__half>(a, st);
 }
 
-// By rows per weight matrix (experts without rows unknown): at 22 rows per expert the tcgen05
-// kernel took 44 us where the one above took 122.
+// Few rows go to the kernel above, which reads the weights once per eight rows; the tcgen05
+// kernel reads them once, but dequantizes no more than 2.3 TB/s of them and takes 12 to 18 us at
+// the least. One pass over the weights is always better with the first (12288x2048 at 8 rows
+// 9.0 against 12.8 us); more passes as long as they are short (16 rows 12.1 against 12.8, 24
+// rows 13.8 against 13.2; 5120x2048 at 32 rows 11.4 against 13.0, at 48 13.6 against 13.3;
+// 2048x4096 at 64 rows 15.4 against 19.3, at 96 21.2 against 20.5; 64 experts of 1536x2048 at 8
+// rows each 47.7 against 49.7, at 12 60.8 against 50.4).
 bool matmul_takes_tc(int R, int E, int N) {
-  if (const char* f = getenv("MM_FORCE")) return f[0] == 't';
-  return matmul_tc_fits(E, N) && R >= 16ll * std::min(E, R);
+  return matmul_tc_fits(E, N) && R > 8ll * std::min(E, R) && (R + 7) / 8 * (long long)N > 25000;
 }
 
 int launch_matmul(const MatmulArgs& a, cudaStream_t st) {
