@@ -115,15 +115,6 @@ struct Conv<__half> {
   }
 };
 
-// tile of `map` at (column, row) into shared memory
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int col, int row,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(bar)
-      : "memory");
-}
 // a 16-bit value in both halves
 __device__ __forceinline__ uint32_t lds_u16x2(uint32_t at) {
   uint16_t v;
@@ -142,12 +133,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-// one lane of a converged warp
-__device__ __forceinline__ bool elect_one() {
+// 1 for one lane of a converged warp, the same each time
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(p));
-  return p != 0;
+  return p;
 }
 
 // Barrier waits by shared address: one poll inline; a wait that lasts suspends in hardware
@@ -207,31 +198,50 @@ __device__ __forceinline__ bool wait_three(uint32_t b1, uint32_t p1, uint32_t b2
   return wait_warp(b1, p1, status, where) && wait_warp(b2, p2, status, where + 10) &&
          wait_warp(b3, p3, status, where + 11);
 }
-__device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes) {
+// The following act for the threads whose `on` is not 0, by predicate: a branch around them
+// costs over a hundred clocks of convergence bookkeeping.
+__device__ __forceinline__ void arrive(uint32_t bar, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(
-          bar),
-      "r"(bytes)
+      "{\n\t.reg .pred q;\n\t.reg .b64 st;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q mbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar),
+      "r"(on)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
+__device__ __forceinline__ void arrive_tx(uint32_t bar, uint32_t bytes, uint32_t on) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      "{\n\t.reg .pred q;\n\t.reg .b64 st;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(on)
+      : "memory");
+}
+// tile of `map` at (column, row) into shared memory
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int col, int row,
+                                          uint32_t bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(bar), "r"(on)
       : "memory");
 }
 // four MMAs of 16 K values: A from tensor memory, B's descriptor by halves
 __device__ __forceinline__ void mma4(uint32_t acc, uint32_t at, uint32_t blo, uint32_t bhi,
-                                     uint32_t idesc, uint32_t accumulate) {
+                                     uint32_t idesc, uint32_t accumulate, uint32_t on) {
 #pragma unroll
   for (int s = 0; s < 4; ++s)
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 d;\n\tmov.b64 d, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, p;\n\t}" ::"r"(acc),
-        "r"(at + s * 8), "r"(blo + s * 2), "r"(bhi), "r"(idesc), "r"(s ? 1u : accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 d;\n\tmov.b64 d, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, p;\n\t}" ::"r"(acc),
+        "r"(at + s * 8), "r"(blo + s * 2), "r"(bhi), "r"(idesc), "r"(s ? 1u : accumulate), "r"(on)
         : "memory");
 }
 
@@ -393,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   // two stages of codes, which count the double steps of their turn.
   const uint32_t bar_a = smem_u32(bars), bar_freed = bar_a + 8 * kBarFreed, bar_b = bar_a + 8 * kBarB, bar_c = bar_a + 8 * kBarC;
   const uint32_t bar_s = bar_a + 8 * kBarS, bar_acc = bar_a + 8 * kBarAcc, bar_fin = bar_a + 8 * kBarFin;
+  const uint32_t one = elect_one();
   bool ok = true;
 
   if (warp >= 4 && warp < 20) {
@@ -407,7 +418,6 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     const uint32_t my_a = tmem + kACol + turn * 64 + h * 32 + ((uint32_t)(q * 32) << 16);
     const uint32_t my_full = bar_a + 8 * (turn * 2 + h), my_freed = bar_freed + 8 * turn;
     const uint32_t my_codes = bar_c + 32 * turn;
-    const bool one = lane == 0;
     uint32_t n = 0, piece = 0;  // double steps of this turn, pieces of scales so far
     while (cur.valid() && ok) {
       for (int k0 = 0; k0 < steps; k0 += kScaleGroups, ++piece) {
@@ -447,14 +457,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           __syncwarp();
           // the codes are freed after their last use, not after their loads: a load that the
           // assembler moved below the arrive would read the stage's next contents
-          if (one) {
-            arrive(my_full);
-            arrive(my_codes + 16 * slot + 8);
-          }
+          arrive(my_full, one);
+          arrive(my_codes + 16 * slot + 8, one);
         }
         if (!ok) break;
         __syncwarp();
-        if (one) arrive(s_bar + 8);
+        arrive(s_bar + 8, one);
       }
       cur.next();
     }
@@ -501,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       }
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive(bar_acc + 16 * buf + 8);
+      arrive(bar_acc + 16 * buf + 8, one);
       ++tile;
       cur.next();
     }
@@ -566,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_s + 16 * buf)
                        : "memory");
         else
-          arrive(bar_s + 16 * buf);
+          arrive(bar_s + 16 * buf, 1);
         buf ^= 1;
         ph ^= buf ^ 1;
       }
@@ -585,11 +593,9 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
         if (!ok) break;
         const uint32_t dst = base + st * 2 * half_bytes, bar = bar_b + 16 * st;
         const bool both = k + 1 < steps;
-        if (elect_one()) {
-          arrive_tx(bar, both ? 2 * half_bytes : half_bytes);
-          load_tile(dst, &p.x, k * 64, row0, bar);
-          if (both) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar);
-        }
+        arrive_tx(bar, both ? 2 * half_bytes : half_bytes, one);
+        load_tile(dst, &p.x, k * 64, row0, bar, one);
+        if (both) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar, one);
         ++issued;
         if (++st == p.b_stages) {
           st = 0;
@@ -619,16 +625,14 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
             const uint32_t dst = base + slot * kSlotBytes, bar = bar_c + 16 * slot;
             ok = wait_warp(bar + 8, (n[turn] >> 1 & 1) ^ 1, a.status, 69);
             if (ok) {
-              if (elect_one()) {
-                arrive_tx(bar, kSlotBytes);
-                if (GATED) {
+              arrive_tx(bar, kSlotBytes, one);
+              if (GATED) {
 #pragma unroll
-                  for (int i = 0; i < 8; ++i)  // 16 gate rows, their 16 up rows, per quarter
-                    load_tile(dst + i * 1024, &p.codes, kk * 32,
-                              row + (i >> 1) * 16 + (i & 1) * n_out, bar);
-                } else {
-                  load_tile(dst, &p.codes, kk * 32, row, bar);
-                }
+                for (int i = 0; i < 8; ++i)  // 16 gate rows, their 16 up rows, per quarter
+                  load_tile(dst + i * 1024, &p.codes, kk * 32,
+                            row + (i >> 1) * 16 + (i & 1) * n_out, bar, one);
+              } else {
+                load_tile(dst, &p.codes, kk * 32, row, bar, one);
               }
               ++n[turn];
             }
@@ -678,25 +682,20 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           bph ^= 1;
         }
         const uint32_t na = bar_a + 16 * turn, nph = aph >> turn & 1;
-        ready = 1;
-        if (elect_one()) {
-          mma4(acc, am, b_at, dhi, idesc, k > 0 ? 1u : 0u);
-          if (k + 1 < steps) mma4(acc, am + 32, b_at + dhalf, dhi, idesc, 1u);
-          // by now the stages freed by the double step before have been refilled
-          ready = test(bb, bph) & test(na, nph) & test(na + 8, nph);
-          commit(freed);
-          commit(b_free);
-          if (last) commit(bar_acc + 16 * buf);
-        }
-        __syncwarp();
+        mma4(acc, am, b_at, dhi, idesc, k > 0 ? 1u : 0u, one);
+        if (k + 1 < steps) mma4(acc, am + 32, b_at + dhalf, dhi, idesc, 1u, one);
+        // by now the stages freed by the double step before have been refilled
+        ready = test(bb, bph) & test(na, nph) & test(na + 8, nph);
+        commit(freed, one);
+        commit(b_free, one);
+        if (last) commit(bar_acc + 16 * buf, one);
       }
       ++tile;
       cur.next();
     }
     // every MMA has completed before tensor memory is freed (one lane, the same each time,
     // issued them all)
-    if (elect_one()) commit(bar_fin);
-    __syncwarp();
+    commit(bar_fin, one);
     wait_warp(bar_fin, 0, a.status, 66);
   }
   tc::fence_before_sync();
