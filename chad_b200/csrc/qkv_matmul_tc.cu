@@ -10,8 +10,9 @@
 //
 //   * Persistent CTAs, one per SM. A tile is (expert, up to 192 of its rows, 128 weight rows);
 //     an expert's rows are cut into equal tiles. Every CTA takes a contiguous range of the
-//     tiles of equal summed cost, computed by each CTA from the offsets: nothing is counted
-//     through memory, and neighbouring tiles share rows of x in L2.
+//     tiles, equally many (a tile takes the dequantizers about the same time whatever its rows),
+//     computed by each CTA from the offsets: nothing is counted through memory, and
+//     neighbouring tiles share rows of x in L2.
 //   * Warps: 0 issues the MMAs, 1 loads rows of x (TMA), 2 packed codes (TMA), 3 scales, 4-19
 //     dequantize (four warpgroups: the two halves of 128 K values, two such in turn), 20-23
 //     store results.
@@ -65,10 +66,6 @@ struct TcArgs {
   int n_tiles;   // tiles of 128 weight rows
 };
 
-// Cost of a tile in units of 16 rows' MMAs: below kMinCost the dequantizers set the pace.
-constexpr int kMinCost = 6;
-constexpr int kFixCost = 1;
-
 struct Split {
   int n;    // row tiles of an expert
   int per;  // rows of each (a multiple of 16; the last may have fewer)
@@ -79,11 +76,6 @@ __host__ __device__ inline Split split_rows(int count, int tok) {
   const int per = ((count + n - 1) / n + 15) / 16 * 16;
   return {(count + per - 1) / per, per};
 }
-__host__ __device__ inline int tile_cost(int per) {
-  const int c = per / 16;
-  return (c > kMinCost ? c : kMinCost) + kFixCost;
-}
-
 template <typename T>
 struct Conv;
 template <>
@@ -252,20 +244,19 @@ struct Cursor {
   long long pos, end;
   int e, seg, j;
   Split s;
-  int cost, row_begin, row_end;
+  int row_begin, row_end;
 
   __device__ __forceinline__ void set_expert() {
     const int lo = __shfl_sync(0xffffffffu, off[e], 0), hi = __shfl_sync(0xffffffffu, off[e + 1], 0);
     row_begin = lo;
     row_end = hi;
     s = split_rows(hi - lo, tok);
-    cost = tile_cost(s.per);
   }
   __device__ __forceinline__ bool valid() const { return e < E && pos < end; }
   __device__ __forceinline__ int row0() const { return row_begin + seg * s.per; }
   __device__ __forceinline__ int row1() const { return min(row_end, row0() + s.per); }
   __device__ __forceinline__ void next() {
-    pos += cost;
+    ++pos;
     if (++j == n_tiles) {
       j = 0;
       if (++seg == s.n) {
@@ -329,11 +320,11 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     off[e] = a.offsets ? min(max(a.offsets[e], 0), a.R) : (e ? a.R : 0);
   __syncthreads();
   if (warp == 3) {
-    // total cost, then the first tile that starts inside this CTA's share
+    // the number of tiles, then the first one of this CTA's share
     long long total = 0;
     for (int e = lane; e < a.E; e += 32) {
       const Split s = split_rows(off[e + 1] - off[e], p.tok);
-      total += (long long)s.n * p.n_tiles * tile_cost(s.per);
+      total += (long long)s.n * p.n_tiles;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -344,8 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       const int e = e0 + lane;
       Split s = {0, 16};
       if (e < a.E) s = split_rows(off[e + 1] - off[e], p.tok);
-      const int c = tile_cost(s.per);
-      const long long mine = (long long)s.n * p.n_tiles * c;
+      const long long mine = (long long)s.n * p.n_tiles;
       long long sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -353,9 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
         if (lane >= o) sum += v;
       }
       const long long begin = base + sum - mine;
-      // index of the first tile of this expert starting at or after lo
-      const long long first = lo > begin ? (lo - begin + c - 1) / c : 0;
-      const bool here = first < (long long)s.n * p.n_tiles;
+      const long long first = lo > begin ? lo - begin : 0;  // tile of this expert
+      const bool here = first < mine;
       const unsigned m = __ballot_sync(0xffffffffu, here);
       if (m) {
         found = true;
@@ -363,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           start_sh[0] = e;
           start_sh[1] = (int)(first / p.n_tiles);
           start_sh[2] = (int)(first % p.n_tiles);
-          range_sh[0] = begin + first * c;
+          range_sh[0] = begin + first;
           range_sh[1] = hi;
         }
       }
@@ -769,17 +758,16 @@ int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st) {
     p.a.rows = nullptr;
   }
   p.n_tiles = gated ? (n_out + 63) / 64 : (n_out + 127) / 128;
-  // One matrix: the row tile that leaves the fewest idle SMs in the last wave. Experts: the
-  // counts are on the device, so the largest.
+  // One matrix: the largest row tile, or a smaller one if that takes fewer rounds of tiles.
+  // Experts: the counts are on the device, so the largest.
   p.tok = kMaxTok;
   if (!a.offsets) {
     long long best = -1;
-    for (int tok = kMaxTok; tok >= 16; tok -= 16) {
+    for (int tok = kMaxTok; tok >= 64; tok -= 16) {
       const Split s = split_rows(a.R, tok);
-      const long long tiles = (long long)s.n * p.n_tiles;
-      const long long cost = (tiles + sms - 1) / sms * tile_cost(s.per);
-      if (best < 0 || cost < best) {
-        best = cost;
+      const long long rounds = ((long long)s.n * p.n_tiles + sms - 1) / sms;
+      if (best < 0 || rounds < best) {
+        best = rounds;
         p.tok = tok;
       }
     }
