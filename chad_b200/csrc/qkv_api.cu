@@ -491,7 +491,7 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
 
 size_t qkv_matmul_workspace_size(int R, int E, int N, int K, int gathered) {
   if (R <= 0 || E <= 0 || N <= 0 || K <= 0 || !gathered) return 0;
-  return matmul_takes_tc(R, E, N) ? matmul_tc_workspace(R, K) : 0;
+  return matmul_takes_tc(R, E, N, K) ? matmul_tc_workspace(R, K) : 0;
 }
 
 int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void* scales,
@@ -537,8 +537,7 @@ int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int norma
     return fail(QKV_EINVAL, "bad sizes T=%d E=%d k=%d", T, E, k);
   if (E > 512 || k > 16)
     return fail(QKV_EUNSUPPORTED, "at most 512 experts and 16 choices (got %d, %d)", E, k);
-  if ((long long)T * k > 0x7fffffffll)
-    return fail(QKV_EUNSUPPORTED, "T * k exceeds 32-bit positions (T=%d k=%d)", T, k);
+  if (T > 1 << 24) return fail(QKV_EUNSUPPORTED, "at most %d tokens (got %d)", 1 << 24, T);
   if (!offsets || (T > 0 && (!logits || !experts || !weights || !rows || !slots)))
     return fail(QKV_EINVAL, "null pointer");
   if (!aligned(logits, dtype == QKV_F32 ? 4 : 2) || !aligned(experts, 4) ||

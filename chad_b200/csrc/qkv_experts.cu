@@ -171,6 +171,7 @@ template <int DTYPE>
 __global__ void __launch_bounds__(kChooseThreads, 2) route_choose_kernel(const RouteArgs a, int bt) {
   extern __shared__ int smem[];
   const int t0 = blockIdx.x * bt, t1 = min(t0 + bt, a.T);
+  wait_for_previous();
   for (int e = threadIdx.x; e < a.E; e += kChooseThreads) smem[e] = 0;
   route_block<DTYPE, kChooseThreads>(a, t0, t1);
   __syncthreads();
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   uint32_t* mask = (uint32_t*)(smem + 2 * a.E + 1);  // words x E
   const int t0 = ONE ? 0 : blockIdx.x * bt, t1 = min(t0 + bt, a.T);
   for (int i = threadIdx.x; i < words * a.E; i += kRouteThreads) mask[i] = 0;
+  wait_for_previous();
   if (ONE) {
     route_block<DTYPE, kRouteThreads>(a, t0, t1);
   } else {
@@ -272,6 +274,7 @@ __global__ void __launch_bounds__(256)
                           const float* __restrict__ weights, const T* __restrict__ residual,
                           T* __restrict__ out, long long n_vec, int per_row, int k, int N) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  wait_for_previous();
   if (i >= n_vec) return;
   const long long t = i / per_row;
   const int c = (int)(i - t * per_row) * VEC;
@@ -331,13 +334,9 @@ int launch_combine_t(const void* y, int R, const int* slots, const float* weight
   const long long n = (long long)tokens * per_row;
   const long long blocks = (n + 255) / 256;
   if (blocks > 0x7fffffffll) return QKV_EUNSUPPORTED;
-  if (vec)
-    expert_combine_kernel<T, 8><<<(unsigned)blocks, 256, 0, st>>>(
-        (const T*)y, R, slots, weights, (const T*)residual, (T*)out, n, per_row, k, N);
-  else
-    expert_combine_kernel<T, 1><<<(unsigned)blocks, 256, 0, st>>>(
-        (const T*)y, R, slots, weights, (const T*)residual, (T*)out, n, per_row, k, N);
-  return QKV_OK;
+  return launch(true, vec ? expert_combine_kernel<T, 8> : expert_combine_kernel<T, 1>,
+                          dim3((unsigned)blocks), 256, 0, st, y, R, slots, weights, residual, out, n,
+                          per_row, k, N);
 }
 
 }  // namespace
@@ -351,9 +350,8 @@ size_t route_workspace_bytes(int T, int E) {
 template <int DTYPE>
 static int launch_route_t(const RouteArgs& a, cudaStream_t st) {
   if (a.T <= kOneBlock) {
-    route_place_kernel<true, DTYPE>
-        <<<1, kRouteThreads, place_smem(a.E, kOneBlock), st>>>(a, kOneBlock, 0);
-    return QKV_OK;
+    return launch(true, route_place_kernel<true, DTYPE>, dim3(1), kRouteThreads,
+                            place_smem(a.E, kOneBlock), st, a, kOneBlock, 0);
   }
   const int bt = route_block_tokens(a.T), place = bt * kPlaceBlocks;
   const unsigned blocks = (unsigned)((a.T + bt - 1) / bt);
@@ -362,11 +360,12 @@ static int launch_route_t(const RouteArgs& a, cudaStream_t st) {
       cudaFuncSetAttribute(route_place_kernel<false, QKV_F32>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return QKV_ECUDA;
-  route_choose_kernel<DTYPE><<<blocks, kChooseThreads, a.E * sizeof(int), st>>>(a, bt);
-  route_place_kernel<false, QKV_F32>
-      <<<(blocks + kPlaceBlocks - 1) / kPlaceBlocks, kRouteThreads, smem, st>>>(a, place,
-                                                                                (int)blocks);
-  return QKV_OK;
+  const int rc = launch(true, route_choose_kernel<DTYPE>, dim3(blocks), kChooseThreads,
+                                  a.E * sizeof(int), st, a, bt);
+  if (rc) return rc;
+  return launch(false, route_place_kernel<false, QKV_F32>,
+                          dim3((blocks + kPlaceBlocks - 1) / kPlaceBlocks), kRouteThreads, smem, st,
+                          a, place, (int)blocks);
 }
 
 int launch_route(const RouteArgs& a, cudaStream_t st) {

@@ -150,10 +150,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][kWarps][4][32];
   __shared__ int seg[3];
-  // what follows in the stream may be set up meanwhile; everything here may come from the
-  // kernel before, the weights too, so nothing is read before it is done
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // everything here may come from the kernel before, the weights too
+  wait_for_previous();
   const MatmulArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -392,19 +390,7 @@ int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
       return QKV_ECUDA;
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, matmul_rows_kernel<T, GATED, SB>, p) == cudaSuccess
-             ? QKV_OK
-             : QKV_ECUDA;
+  return launch(true, matmul_rows_kernel<T, GATED, SB>, grid, kWarps * 32, smem, st, p);
 }
 
 template <typename T, bool GATED>
@@ -473,12 +459,14 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
 // rows 13.8 against 13.2; 5120x2048 at 32 rows 11.4 against 13.0, at 48 13.6 against 13.3;
 // 2048x4096 at 64 rows 15.4 against 19.3, at 96 21.2 against 20.5; 64 experts of 1536x2048 at 8
 // rows each 47.7 against 49.7, at 12 60.8 against 50.4).
-bool matmul_takes_tc(int R, int E, int N) {
-  return matmul_tc_fits(E, N) && R > 8ll * std::min(E, R) && (R + 7) / 8 * (long long)N > 25000;
+bool matmul_takes_tc(int R, int E, int N, int K) {
+  if (!matmul_tc_fits(E, N)) return false;
+  if (K > 65536) return true;  // a row of x does not fit shared memory beside the rings above
+  return R > 8ll * std::min(E, R) && (R + 7) / 8 * (long long)N > 25000;
 }
 
 int launch_matmul(const MatmulArgs& a, cudaStream_t st) {
-  if (matmul_takes_tc(a.R, a.E, a.N)) return launch_matmul_tc(a, st);
+  if (matmul_takes_tc(a.R, a.E, a.N, a.K)) return launch_matmul_tc(a, st);
   return launch_matmul_rows(a, st);
 }
 

@@ -64,6 +64,7 @@ struct TcArgs {
   int tok;       // most rows of x per tile (a multiple of 16)
   int b_stages;
   int n_tiles;   // tiles of 128 weight rows
+  bool gathered; // rows of x by gather_rows_kernel just before
 };
 
 struct Split {
@@ -312,6 +313,9 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     mbar_init(&bars[kBarFin], 1);
     fence_mbar_init();
   }
+  // Tensor memory is taken after the kernel before has ended and before the next one may be set
+  // up: neither can hold columns that this one waits for while it waits for this one.
+  wait_for_kernel_before();
   if (warp == 0) {
     tc::tmem_alloc(&tmem_sh, 512);
     tc::tmem_relinquish();
@@ -366,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  allow_next_kernel();
   const uint32_t tmem = tmem_sh;
   Cursor cur;
   cur.off = off;
@@ -701,6 +706,7 @@ __global__ void __launch_bounds__(256)
     gather_rows_kernel(const uint4* __restrict__ x, long long ldx, int x_rows,
                        const int* __restrict__ rows, uint4* __restrict__ out, int R, int per_row) {
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  wait_for_previous();
   if (r >= R) return;
   const int from = rows[r];
   const bool in = from >= 0 && from < x_rows;
@@ -731,8 +737,7 @@ int launch_tc_t(TcArgs& p, int grid, cudaStream_t st) {
                      GATED ? 16 : 128) ||
       !make_rows_map(&p.x, p.a.x, 2, p.a.K, p.a.x_rows, p.a.ldx * 2, 64, p.tok))
     return QKV_ECUDA;
-  matmul_tc_kernel<T, GATED><<<grid, kThreads, smem, st>>>(p);
-  return QKV_OK;
+  return launch(!p.gathered, matmul_tc_kernel<T, GATED>, dim3(grid), kThreads, smem, st, p);
 }
 
 }  // namespace
@@ -749,9 +754,11 @@ int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st) {
   const int sms = num_sms();
   TcArgs p;
   p.a = a;
+  p.gathered = a.rows != nullptr;
   if (a.rows) {
-    gather_rows_kernel<<<(a.R + 7) / 8, 256, 0, st>>>((const uint4*)a.x, a.ldx / 8, a.x_rows,
-                                                      a.rows, (uint4*)a.workspace, a.R, a.K / 8);
+    const int rc = launch(true, gather_rows_kernel, dim3((a.R + 7) / 8), 256, 0, st, a.x,
+                                    a.ldx / 8, a.x_rows, a.rows, a.workspace, a.R, a.K / 8);
+    if (rc) return rc;
     p.a.x = a.workspace;
     p.a.ldx = a.K;
     p.a.x_rows = a.R;

@@ -284,7 +284,7 @@ int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows
                        void* stream);
 
 /*
- * Route T tokens to k of E experts (E <= 512, k <= 16, k <= E): logits (T, E) in `dtype`
+ * Route T <= 2^24 tokens to k of E experts (E <= 512, k <= 16, k <= E): logits (T, E) in `dtype`
  * (bf16, f16 or f32). experts, weights (T, k): the k largest logits in descending order (ties
  * to the lowest expert; a NaN counts as the largest and makes its token's weights NaN) and
  * their softmax over all E logits, or over the chosen k with normalize != 0; an expert whose

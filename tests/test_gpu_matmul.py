@@ -72,6 +72,8 @@ MATMUL = [
     (1, 40000, 128), (5, 20001, 320), (40, 9000, 192),
     # more K than any ring of shared-memory stages holds, twice over
     (3, 1000, 4096), (33, 600, 6144), (200, 1300, 4096), (192, 130, 6208),
+    # K that leaves shared memory for eight, three, one and no row of x
+    (9, 20, 8192), (9, 20, 20480), (3, 20, 65536), (2, 20, 65600),
 ]
 
 

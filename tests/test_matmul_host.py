@@ -59,7 +59,7 @@ def _route(lib, **over):
     (dict(E=0), EINVAL), (dict(T=-1), EINVAL), (dict(dtype=3), EINVAL), (dict(logits=None), EINVAL),
     (dict(offsets=None), EINVAL), (dict(experts=None), EINVAL), (dict(weights=18), EALIGN),
     (dict(logits=17), EALIGN), (dict(T=1000, ws=None), EWS), (dict(T=1000, ws_bytes=64), EWS),
-    (dict(T=1000, ws=20), EALIGN), (dict(T=1 << 28, k=16), EUNSUP),
+    (dict(T=1000, ws=20), EALIGN), (dict(T=(1 << 24) + 1), EUNSUP),
 ])
 def test_route_rejects_bad_arguments(over, code):
     assert _route(_lib.load(), **over) == code
