@@ -8,7 +8,7 @@
 // and nothing of the weight is rounded. The A operand holds 16 weight rows, the B operand up
 // to 8 rows of x. Codes enter the MMA without a conversion: in bf16 as 128 + code (the code
 // is the low mantissa bits of 128.0; the 128 * sum_k x is taken off with the bias), in f16 as
-// the subnormal code * 2^-24 (the scale carries the 2^24). sum_k x comes from the same tensor
+// the subnormal code * 2^-24 (taken out of the result). sum_k x comes from the same tensor
 // pipe with a matrix of ones.
 //
 // K order. A 32-bit word holds codes k..k+7 LSB-first, and one shift-and-mask yields the pair
@@ -34,35 +34,43 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kChunk = 256;  // K values per warp step: four groups, one per lane of a quad
 
+// D = A B or D += A B, m16n8k16 with fp32 sums
+#define QKV_MMA16(TYPE)                                                                          \
+  static __device__ __forceinline__ void mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, \
+                                              uint32_t b1) {                                      \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                           \
+                 ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"              \
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                 \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));       \
+  }                                                                                               \
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,  \
+                                             uint32_t b1) {                                       \
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                           \
+                 ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"                  \
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                 \
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                 \
+  }
+
 template <typename T>
 struct Codes;
 template <>
 struct Codes<__nv_bfloat16> {
   static constexpr uint32_t kMagic = 0x43004300u;  // 128.0 | code
   static constexpr uint32_t kOnes = 0x3f803f80u;
-  // scale of the accumulated sum, and bias of the x sum
-  static __device__ __forceinline__ float scale(float s) { return s; }
+  static constexpr float kUnit = 1.f;  // what a code of 1 counts in the MMA
+  // factor of the sum of x beside the scale's sum of codes
   static __device__ __forceinline__ float bias(float s, float b) { return fmaf(-128.f, s, b); }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
+  QKV_MMA16("bf16")
 };
 template <>
 struct Codes<__half> {
   static constexpr uint32_t kMagic = 0u;  // the code as an f16 subnormal: code * 2^-24
   static constexpr uint32_t kOnes = 0x3c003c00u;
-  static __device__ __forceinline__ float scale(float s) { return s * 16777216.f; }
+  static constexpr float kUnit = 1.f / 16777216.f;
   static __device__ __forceinline__ float bias(float, float b) { return b; }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    mma16816(d, a, b0, b1);
-  }
+  QKV_MMA16("f16")
 };
+#undef QKV_MMA16
 
 __device__ __forceinline__ uint2 lds_v2(uint32_t at) {
   uint2 v;
@@ -131,10 +139,10 @@ constexpr int kStages = 3;                  // of one chunk, per warp
 constexpr int kCodeBytes = 16 * 128;        // 16 weight rows
 constexpr int kStageBytes = kCodeBytes + 2 * 16 * 8;  // and four scales and biases of each
 
-// Dynamic shared memory of a CTA (8 KiB of sums are static): rows of x and their sums by group,
-// then the rings.
+// Dynamic shared memory of a CTA (8 KiB of sums are static): rows of x, their sums by group and
+// a row of zeros, then the rings.
 constexpr int kDynamicBytes = 227 * 1024 - 8192 - 256;
-inline long long x_bytes(int rows, int K) { return (long long)rows * K * 2 + (long long)K / 64 * 32; }
+inline long long x_bytes(int rows, int K) { return (long long)rows * K * 2 + (long long)K / 64 * 32 + 128; }
 
 struct RowsArgs {
   MatmulArgs a;
@@ -184,7 +192,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const int units = (p.tiles + wn_count - 1) / wn_count;  // of wn_count tiles
   const uint32_t xs = smem_u32(smem);
   const uint32_t sums = xs + (uint32_t)rows * a.K * 2;  // of each group of each row of x
-  const uint32_t ring = sums + (uint32_t)G * 32 + warp * kStages * kStageBytes;
+  const uint32_t zeros = sums + (uint32_t)G * 32;         // what rows past the last read
+  const uint32_t ring = zeros + 128 + warp * kStages * kStageBytes;
 
   // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
   // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
@@ -193,40 +202,40 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
                         : min(tile * 16 + r, n_out - 1);
     return (long long)expert * a.N + n;
   };
-  int ld_unit = blockIdx.x, ld_c = wk, ld_slot = 0;
-  const char* src[4];   // this lane's 16 bytes of rows lane/8 + 4i
-  const char* ssrc;     // scales of row lane (biases of row lane - 16)
+  int ld_unit = blockIdx.x, ld_c = wk;
+  const char* src[4];  // this lane's 16 bytes of rows lane/8 + 4i of the next chunk
+  const char* ssrc;    // scales of row lane (biases of row lane - 16)
   auto set_src = [&]() {
-    const int tile = min(ld_unit * wn_count + wn, p.tiles - 1);
+    const int ld_tile = min(ld_unit * wn_count + wn, p.tiles - 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      src[i] = (const char*)a.w + weight_row(tile, (lane >> 3) + 4 * i) * (a.K / 2) + (lane & 7) * 16;
-    ssrc = (const char*)(lane < 16 ? a.scales : a.biases) + weight_row(tile, lane & 15) * G * 2;
+      src[i] = (const char*)a.w + weight_row(ld_tile, (lane >> 3) + 4 * i) * (a.K / 2) + ld_c * 128 +
+               (lane & 7) * 16;
+    ssrc = (const char*)(lane < 16 ? a.scales : a.biases) + weight_row(ld_tile, lane & 15) * G * 2 +
+           ld_c * 8;
   };
   set_src();
+  // rows lane/8 + 4i, a 512-byte step (the swizzle keeps the fragment reads apart); scales
+  const uint32_t code_to = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) & 3) << 1) << 4);
+  const uint32_t scale_to = ring + kCodeBytes + lane * 8;
+  uint32_t ld_at = 0;  // the stage's offset
   auto load = [&]() {
-    if (ld_unit < units && ld_c < chunks) {
-      const uint32_t at = ring + ld_slot * kStageBytes;
+    if (ld_unit < units) {
       if (ld_c * 8 + (lane & 7) < pieces) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (lane >> 3) + 4 * i;  // (the swizzle keeps the fragment reads apart)
-          cp16(at + r * 128 + (((lane & 7) ^ (r & 3) << 1) << 4), src[i] + (long long)ld_c * 128);
-        }
+        for (int i = 0; i < 4; ++i) cp16(code_to + ld_at + i * 512, src[i]);
       }
-      const uint32_t to = at + kCodeBytes + lane * 8;
-      const char* from = ssrc + ld_c * 8;
       if (SB == 2) {
-        cp_small<8>(to, from);
+        cp_small<8>(scale_to + ld_at, ssrc);
       } else if (SB == 1) {
-        cp_small<4>(to, from);
-        if (ld_c * 4 + 2 < G) cp_small<4>(to + 4, from + 4);
+        cp_small<4>(scale_to + ld_at, ssrc);
+        if (ld_c * 4 + 2 < G) cp_small<4>(scale_to + ld_at + 4, ssrc + 4);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (ld_c * 4 + j < G) {
-            const uint16_t v = __ldg((const uint16_t*)from + j);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 2 * j), "h"(v) : "memory");
+            const uint16_t v = __ldg((const uint16_t*)ssrc + j);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_to + ld_at + 2 * j), "h"(v) : "memory");
           }
       }
       ld_c += wk_count;
@@ -234,9 +243,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         ld_c = wk;
         ld_unit += gridDim.x;
         set_src();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) src[i] += wk_count * 128;
+        ssrc += wk_count * 8;
       }
     }
-    ld_slot = ld_slot + 1 == kStages ? 0 : ld_slot + 1;
+    ld_at = ld_at + kStageBytes == kStages * kStageBytes ? 0 : ld_at + kStageBytes;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
@@ -260,54 +273,73 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
     sts_v4(to + (~m & 1) * 16, make_uint4(prmt(v.x, v.z, 0x5410), prmt(v.x, v.z, 0x7632),
                                           prmt(v.y, v.w, 0x5410), prmt(v.y, v.w, 0x7632)));
   }
+  if (threadIdx.x < 8) sts_v4(zeros + threadIdx.x * 16, make_uint4(0, 0, 0, 0));
   __syncthreads();
 
-  // one group of x as B fragments: lane (g, t) holds 16 values of row g of each tile
-  const uint32_t my_x = xs + g * 128 + t * 32;
-  auto x_frag = [&](int group, uint4 (&xv)[2]) {
-    xv[0] = xv[1] = make_uint4(0, 0, 0, 0);
-    if (g < rows) {
-      const uint32_t xa = my_x + group * rows * 128;
-      xv[0] = lds_v4(xa + (g & 1) * 16);
-      xv[1] = lds_v4(xa + (~g & 1) * 16);
-    }
+  // one group of x as B fragments: lane (g, t) holds 16 values of row g
+  const uint32_t my_x = (g < rows ? xs + g * 128 : zeros) + t * 32, x_step = g < rows ? rows * 128 : 0;
+  auto x_frag = [&](uint32_t at, uint4 (&xv)[2]) {
+    xv[0] = lds_v4(at + (g & 1) * 16);
+    xv[1] = lds_v4(at + (~g & 1) * 16);
   };
-  // sums of x by group, with a matrix of ones
+  // sums of x by group, with a matrix of ones, in the unit of the codes' sums
   for (int j = warp; j < G; j += kWarps) {
     const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes};
     uint4 xv[2];
-    x_frag(j, xv);
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      Codes<T>::mma(d, ones, xv[i].x, xv[i].y);
-      Codes<T>::mma(d, ones, xv[i].z, xv[i].w);
-    }
+    x_frag(my_x + j * x_step, xv);
+    float d[4];
+    Codes<T>::mma0(d, ones, xv[0].x, xv[0].y);
+    Codes<T>::mma(d, ones, xv[0].z, xv[0].w);
+    Codes<T>::mma(d, ones, xv[1].x, xv[1].y);
+    Codes<T>::mma(d, ones, xv[1].z, xv[1].w);
     if (g == 0)
-      asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + j * 32 + t * 8), "f"(d[0]),
-                   "f"(d[1])
+      asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + j * 32 + t * 8), "f"(d[0] * Codes<T>::kUnit),
+                   "f"(d[1] * Codes<T>::kUnit)
                    : "memory");
   }
   __syncthreads();
-  const uint32_t code_at = g * 128 + (t & 1) * 8;
-  int slot = 0, buf = 0;
+  uint32_t code_at[4];  // of the chunk's groups
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    code_at[j] = ring + g * 128 + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4) + (t & 1) * 8;
+  // results of a tile: lane (g, t) holds weight rows g and g + 8 for rows 2t and 2t + 1 of x
+  auto store = [&](int tile, float (&acc)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= 1.f / Codes<T>::kUnit;
+    const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
+    T* out = (T*)a.out;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = t * 2 + i;
+      if (r >= rows) continue;
+      T* o = out + (long long)(row0 + r) * n_out;
+      if (GATED) {
+        const float gate = acc[i], up = acc[i + 2];
+        if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
+      } else {
+        if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[i]);
+        if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[i + 2]);
+      }
+    }
+  };
+  uint32_t at = 0;  // the stage's offset
+  int buf = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int tile = unit * wn_count + wn;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = wk; c < chunks; c += wk_count) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp();
-      const uint32_t at = ring + slot * kStageBytes;
-      slot = slot + 1 == kStages ? 0 : slot + 1;
       load();  // into the stage of the chunk before
       // scales and biases of rows g and g + 8, four groups each
-      const uint2 sA = lds_v2(at + kCodeBytes + g * 8), sB = lds_v2(at + kCodeBytes + 64 + g * 8);
-      const uint2 bA = lds_v2(at + kCodeBytes + 128 + g * 8), bB = lds_v2(at + kCodeBytes + 192 + g * 8);
+      const uint32_t sat = ring + at + kCodeBytes + g * 8;
+      const uint2 sA = lds_v2(sat), sB = lds_v2(sat + 64), bA = lds_v2(sat + 128), bB = lds_v2(sat + 192);
+      uint32_t xa = my_x + c * 4 * x_step;
+      const uint32_t sum_at = sums + c * 128 + t * 8;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (c * 4 + j >= G) break;
-        const uint32_t ca = at + code_at + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4);
-        const uint2 wa = lds_v2(ca), wb = lds_v2(ca + 1024);
+        if (SB != 2 && c * 4 + j >= G) break;  // (SB 2: whole chunks)
+        const uint2 wa = lds_v2(code_at[j] + at), wb = lds_v2(code_at[j] + at + 1024);
         uint32_t f[4][4];  // A fragments of the group's four MMAs
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -321,25 +353,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
         const uint32_t s0 = j < 2 ? sA.x : sA.y, s1 = j < 2 ? sB.x : sB.y;
         const uint32_t b0 = j < 2 ? bA.x : bA.y, b1 = j < 2 ? bB.x : bB.y;
         const int sh = (j & 1) * 16;
-        const float f0 = Elem<T>::bits_to_f32((uint16_t)(s0 >> sh));
-        const float f1 = Elem<T>::bits_to_f32((uint16_t)(s1 >> sh));
-        const float o0 = Codes<T>::bias(f0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
-        const float o1 = Codes<T>::bias(f1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
-        const float q0 = Codes<T>::scale(f0), q1 = Codes<T>::scale(f1);
+        const float q0 = Elem<T>::bits_to_f32((uint16_t)(s0 >> sh));
+        const float q1 = Elem<T>::bits_to_f32((uint16_t)(s1 >> sh));
+        const float o0 = Codes<T>::bias(q0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
+        const float o1 = Codes<T>::bias(q1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
         uint4 xv[2];
-        x_frag(c * 4 + j, xv);
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        Codes<T>::mma(d, f[0], xv[0].x, xv[0].y);
+        x_frag(xa, xv);
+        xa += x_step;
+        float d[4];
+        Codes<T>::mma0(d, f[0], xv[0].x, xv[0].y);
         Codes<T>::mma(d, f[1], xv[0].z, xv[0].w);
         Codes<T>::mma(d, f[2], xv[1].x, xv[1].y);
         Codes<T>::mma(d, f[3], xv[1].z, xv[1].w);
-        const uint2 sx = lds_v2(sums + (c * 4 + j) * 32 + t * 8);
+        const uint2 sx = lds_v2(sum_at + j * 32);
         const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
         acc[0] = fmaf(q0, d[0], fmaf(o0, sx0, acc[0]));
         acc[1] = fmaf(q0, d[1], fmaf(o0, sx1, acc[1]));
         acc[2] = fmaf(q1, d[2], fmaf(o1, sx0, acc[2]));
         acc[3] = fmaf(q1, d[3], fmaf(o1, sx1, acc[3]));
       }
+      at = at + kStageBytes == kStages * kStageBytes ? 0 : at + kStageBytes;
     }
 
     if (wk_count > 1) {
@@ -357,23 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       }
       buf ^= 1;
     }
-    if (wk == 0 && tile < p.tiles) {
-      const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
-      T* out = (T*)a.out;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = t * 2 + i;
-        if (r >= rows) continue;
-        T* o = out + (long long)(row0 + r) * n_out;
-        if (GATED) {
-          const float gate = acc[i], up = acc[i + 2];
-          if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
-        } else {
-          if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[i]);
-          if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[i + 2]);
-        }
-      }
-    }
+    if (wk == 0 && tile < p.tiles) store(tile, acc);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
