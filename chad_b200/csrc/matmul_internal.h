@@ -42,7 +42,7 @@ struct RouteArgs {
   int* rows;           // (T * k) token of each sorted pair
   int* slots;          // (T, k) sorted position of each pair
   int* offsets;        // (E + 1)
-  int* hist;           // workspace: (blocks, E)
+  int* hist;           // workspace: (blocks, (E + 1) / 2) pairs of 16-bit counts
 };
 
 size_t route_workspace_bytes(int T, int E);

@@ -5,8 +5,7 @@
 // sort of the T*k pairs by expert: rows (token of each sorted pair), slots (sorted position
 // of each pair) and offsets (first sorted pair of each expert).
 //
-// One warp per token holds its logits in registers as order-preserving unsigned keys; a
-// selection is one redux.max over the keys and one redux.min over the indices that have it.
+// One warp per token holds its logits in registers as order-preserving unsigned keys.
 // A token takes an expert at most once, so a pair's rank within its expert is the number of
 // earlier tokens that took it: a popcount over a per-expert bit mask of tokens. Counts and
 // masks are integers, so the order of their atomics does not show.
@@ -27,6 +26,7 @@ constexpr int kRouteThreads = 1024;   // of a block that places
 constexpr int kChooseThreads = 512;   // of a block that chooses: two fit an SM
 constexpr int kPlaceBlocks = 4;       // choosing blocks whose pairs one block places
 constexpr int kMaxBlockTokens = 512;
+constexpr int kMaxRouteExperts = 512;
 
 template <int DTYPE>
 __device__ __forceinline__ float load_logit(const void* p, long long i) {
@@ -47,12 +47,16 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key == 0xffffffffu ? 0x7fffffffu : key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// One warp, one token: experts[0..k), weights[0..k). PER = logits per lane. Every lane keeps the
-// best of its own logits; a choice is a redux.max over the lanes' best keys, a redux.min over
-// the indices that have it, and a new best for the lane it came from. The first choice is the
-// softmax's maximum.
+// One warp, one token: experts[0..k), weights[0..k). PER = logits per lane.
+//
+// The k-th largest of the lanes' best keys is a lower bound of the k-th largest key, found by
+// redux.max over one key per lane. What reaches it, a few more than k keys, goes to shared
+// memory in the experts' order, one to a lane, where its rank is the number of those before it:
+// compares that do not wait for one another. (Choosing one after the other among all keys, each
+// time with a new best for the lane it came from, took 17.5 us for 8192 tokens of 256 experts.)
+// Keys in such numbers that 32 lanes do not hold them are chosen one after the other.
 template <int DTYPE, int PER>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane, uint2* held) {
   uint32_t key[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -60,19 +64,9 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int token, int l
     // 0 is below every logit's key (-inf has 0x7fffff)
     key[i] = e < a.E ? order_key(load_logit<DTYPE>(a.logits, (long long)token * a.E + e)) : 0u;
   }
-  uint32_t best;
-  int best_i;
-  auto find_best = [&]() {
-    best = key[0];
-    best_i = 0;
+  uint32_t best = key[0];
 #pragma unroll
-    for (int i = 1; i < PER; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        best_i = i;
-      }
-  };
-  find_best();
+  for (int i = 1; i < PER; ++i) best = max(best, key[i]);
   const uint32_t top = __reduce_max_sync(0xffffffffu, best);
   const float mx = key_value(top);
   float total = 0.f;
@@ -85,33 +79,73 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int token, int l
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  uint32_t at = 0, chosen = 0;  // lane j < k keeps the j-th choice
-#pragma unroll 1
-  for (int j = 0; j < a.k; ++j) {
-    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t mine = best == high ? best_i * 32u + lane : ~0u;
-    const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
-    if (lane == j) {
-      at = e;
-      chosen = high;
-    }
-    // without a branch: the lane of the choice drops it and finds its next best
-    const int drop = e == mine ? best_i : -1;
+  // (at least min(E, 32) >= k lanes have a key, so the bound is a key)
+  uint32_t bound = top;
+  for (int n = 0;;) {
+    n += __popc(__ballot_sync(0xffffffffu, best == bound));
+    if (n >= a.k) break;
+    best = best == bound ? 0u : best;
+    bound = __reduce_max_sync(0xffffffffu, best);
+  }
+  int count = 0;
+  __syncwarp();  // (the token before has been read)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = i == drop ? 0u : key[i];
-    find_best();
+  for (int i = 0; i < PER; ++i) {
+    const bool in = key[i] >= bound;
+    const uint32_t m = __ballot_sync(0xffffffffu, in);
+    const int at = count + __popc(m & ((1u << lane) - 1));
+    if (in && at < 32) held[at] = make_uint2(key[i], i * 32 + lane);
+    count += __popc(m);
+  }
+  __syncwarp();
+  uint32_t chosen = 0, at = 0;  // key and expert of this lane, and where it stands
+  int rank = 32;
+  if (count <= 32) {
+    if (lane < count) {
+      const uint2 c = held[lane];
+      chosen = c.x;
+      at = c.y;
+      rank = 0;
+    }
+#pragma unroll 4
+    for (int c = 0; c < count; ++c) {
+      const uint32_t other = __shfl_sync(0xffffffffu, chosen, c);
+      rank += other > chosen || (other == chosen && c < lane);
+    }
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t b = 0;
+      int b_i = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (key[i] > b) {
+          b = key[i];
+          b_i = i;
+        }
+      const uint32_t high = __reduce_max_sync(0xffffffffu, b);
+      const uint32_t mine = b == high ? b_i * 32u + lane : ~0u;
+      const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
+      if (lane == j) {
+        at = e;
+        chosen = high;
+        rank = j;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = e == mine && i == b_i ? 0u : key[i];
+    }
   }
   const float v = key_value(chosen);
-  const float p = lane >= a.k || v == -INFINITY ? 0.f : expf(v - mx);
+  const float p = rank >= a.k || v == -INFINITY ? 0.f : expf(v - mx);
   if (a.normalize) {
     total = p;
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  if (lane < a.k) {
+  if (rank < a.k) {
     // total is 0 only for a row of -inf, whose weights are 0
-    a.experts[(long long)token * a.k + lane] = (int)at;
-    a.weights[(long long)token * a.k + lane] = total == 0.f ? 0.f : p / total;
+    a.experts[(long long)token * a.k + rank] = (int)at;
+    a.weights[(long long)token * a.k + rank] = total == 0.f ? 0.f : p / total;
   }
 }
 
@@ -119,12 +153,14 @@ template <int DTYPE, int THREADS>
 __device__ __forceinline__ void route_block(const RouteArgs& a, int t0, int t1) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (a.E + 31) / 32;
+  __shared__ uint2 held_of[THREADS / 32][32];
+  uint2* held = held_of[warp];
   for (int t = t0 + warp; t < t1; t += THREADS / 32) {
-    if (per <= 1) route_token<DTYPE, 1>(a, t, lane);
-    else if (per <= 2) route_token<DTYPE, 2>(a, t, lane);
-    else if (per <= 4) route_token<DTYPE, 4>(a, t, lane);
-    else if (per <= 8) route_token<DTYPE, 8>(a, t, lane);
-    else route_token<DTYPE, 16>(a, t, lane);
+    if (per <= 1) route_token<DTYPE, 1>(a, t, lane, held);
+    else if (per <= 2) route_token<DTYPE, 2>(a, t, lane, held);
+    else if (per <= 4) route_token<DTYPE, 4>(a, t, lane, held);
+    else if (per <= 8) route_token<DTYPE, 8>(a, t, lane, held);
+    else route_token<DTYPE, 16>(a, t, lane, held);
   }
 }
 
@@ -178,8 +214,11 @@ __global__ void __launch_bounds__(kChooseThreads, 2) route_choose_kernel(const R
   for (int i = threadIdx.x; i < (t1 - t0) * a.k; i += kChooseThreads)
     atomicAdd(&smem[a.experts[(long long)t0 * a.k + i]], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += kChooseThreads)
-    a.hist[(long long)blockIdx.x * a.E + e] = smem[e];
+  // (a block's count fits 16 bits: every placing block reads all of them)
+  const int words = (a.E + 1) / 2;
+  for (int i = threadIdx.x; i < words; i += kChooseThreads)
+    a.hist[(long long)blockIdx.x * words + i] =
+        smem[2 * i] | (2 * i + 1 < a.E ? smem[2 * i + 1] << 16 : 0);
 }
 
 // Sorted positions of one block's pairs. ONE: a single block that also chooses (a decode
@@ -201,26 +240,35 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
     // the block's threads share the rows of counts of every expert
     for (int e = threadIdx.x; e < a.E; e += kRouteThreads) base[e] = before[e] = 0;
     __syncthreads();
-    const int lanes = (a.E + 31) / 32 * 32, share = kRouteThreads / lanes;
-    const int e = threadIdx.x % lanes, part = threadIdx.x / lanes;
-    if (part < share && e < a.E) {
-      int all = 0, prior = 0;
+    // (words of two counts)
+    const int width = (a.E + 1) / 2, lanes = (width + 31) / 32 * 32, share = kRouteThreads / lanes;
+    const int w = threadIdx.x % lanes, part = threadIdx.x / lanes;
+    if (part < share && w < width) {
+      int all[2] = {0, 0}, prior[2] = {0, 0};
       const int mine = blockIdx.x * kPlaceBlocks;
       for (int b0 = part; b0 < counted; b0 += 16 * share) {
-        int n[16];  // sixteen loads in flight
+        uint32_t n[16];  // sixteen loads in flight
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int b = b0 + i * share;
-          n[i] = b < counted ? __ldg(a.hist + (long long)b * a.E + e) : 0;
+          n[i] = b < counted ? __ldg((const uint32_t*)a.hist + (long long)b * width + w) : 0;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          all += n[i];
-          prior += b0 + i * share < mine ? n[i] : 0;
+          const int lo = n[i] & 0xffff, hi = n[i] >> 16;
+          const bool before_mine = b0 + i * share < mine;
+          all[0] += lo;
+          all[1] += hi;
+          prior[0] += before_mine ? lo : 0;
+          prior[1] += before_mine ? hi : 0;
         }
       }
-      atomicAdd(&base[e], all);
-      atomicAdd(&before[e], prior);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (2 * w + q < a.E) {
+          atomicAdd(&base[2 * w + q], all[q]);
+          atomicAdd(&before[2 * w + q], prior[q]);
+        }
     }
   }
   __syncthreads();
@@ -344,7 +392,7 @@ int launch_combine_t(const void* y, int R, const int* slots, const float* weight
 size_t route_workspace_bytes(int T, int E) {
   if (T <= kOneBlock) return 0;
   const int bt = route_block_tokens(T);
-  return (size_t)((T + bt - 1) / bt) * E * sizeof(int);
+  return (size_t)((T + bt - 1) / bt) * ((E + 1) / 2) * sizeof(int);
 }
 
 template <int DTYPE>
@@ -356,9 +404,12 @@ static int launch_route_t(const RouteArgs& a, cudaStream_t st) {
   const int bt = route_block_tokens(a.T), place = bt * kPlaceBlocks;
   const unsigned blocks = (unsigned)((a.T + bt - 1) / bt);
   const size_t smem = place_smem(a.E, place);
+  // (the bound is the same for every call: another thread's may come before this launch)
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(route_place_kernel<false, QKV_F32>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)place_smem(kMaxRouteExperts, kMaxBlockTokens * kPlaceBlocks)) !=
+          cudaSuccess)
     return QKV_ECUDA;
   const int rc = launch(true, route_choose_kernel<DTYPE>, dim3(blocks), kChooseThreads,
                                   a.E * sizeof(int), st, a, bt);

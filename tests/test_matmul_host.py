@@ -85,10 +85,11 @@ def test_workspace_sizes():
     lib = _lib.load()
     assert lib.qkv_route_workspace_size(0, 64) == 0
     assert lib.qkv_route_workspace_size(64, 64) == 0
-    # blocks of 32 tokens, then larger ones so that 256 blocks are not passed
-    assert lib.qkv_route_workspace_size(65, 64) == 3 * 64 * 4
-    assert lib.qkv_route_workspace_size(8192, 128) == 256 * 128 * 4
-    assert lib.qkv_route_workspace_size(8193, 128) == 129 * 128 * 4
+    # two counts to a word; blocks of 32 tokens, then larger ones so that 256 are not passed
+    assert lib.qkv_route_workspace_size(65, 64) == 3 * 32 * 4
+    assert lib.qkv_route_workspace_size(8192, 128) == 256 * 64 * 4
+    assert lib.qkv_route_workspace_size(8193, 128) == 129 * 64 * 4
+    assert lib.qkv_route_workspace_size(65, 7) == 3 * 4 * 4
 
 
 def test_operators_refuse_cpu_tensors():
