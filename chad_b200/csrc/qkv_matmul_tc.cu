@@ -27,11 +27,11 @@
 // rounding included) against its 1.7e-3, of a gated product by 2.7e-3 against 1.7e-3; in f16 by
 // 2.8e-4 and 3.4e-4 against 2.1e-4. Weights in two terms would double the MMAs and the stores.
 //
-// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 147 us: the tensor pipe is
+// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 143 us: the tensor pipe is
 // busy 47% of the time, the ALU pipe with dequantizing 52% (its warps wait for
 // freed A stages about as often as the MMAs wait for full ones), HBM at 1.8 TB/s. 2048 rows through
 // 5120x2048: 33.6 us, 1280 TFLOP/s, tensor pipe 62 to 76%. Run without a pause both are at the
-// card's power limit (1530 MHz): 172 and 40 us.
+// card's power limit (1550 MHz): 168 and 40 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -51,6 +51,7 @@ namespace {
 constexpr int kWarps = 24;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxTok = 192;           // rows of x in a tile
+constexpr int kBoxRows = 32;           // rows of x are copied in multiples of this
 constexpr int kAStages = 4;            // of 64 K values, in tensor memory
 constexpr int kACol = 2 * kMaxTok;     // first A column
 constexpr int kMaxBStages = 8;         // of 128 K values
@@ -68,7 +69,7 @@ constexpr int kMaxExperts = 1024;
 
 struct TcArgs {
   CUtensorMap codes;  // (E * N, K/2) bytes; boxes of 128 rows, or of 16 gate or up rows
-  CUtensorMap x;      // (x_rows, K); boxes of `tok` rows
+  CUtensorMap x[kMaxTok / kBoxRows];  // (x_rows, K); boxes of 1, 2, ... times kBoxRows rows
   MatmulArgs a;
   int tok;       // most rows of x per tile (a multiple of 16)
   int b_stages;
@@ -86,6 +87,7 @@ __host__ __device__ inline Split split_rows(int count, int tok) {
   const int per = ((count + n - 1) / n + 15) / 16 * 16;
   return {(count + per - 1) / per, per};
 }
+__host__ __device__ inline int stage_rows(int tok) { return (tok + kBoxRows - 1) / kBoxRows * kBoxRows; }
 template <typename T>
 struct Conv;
 template <>
@@ -392,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
                         : min(j * 128 + r, n_out - 1);
     return (long long)e * a.N + n;
   };
-  const int half_bytes = p.tok * 128;  // a B stage is two tiles of 64 K values
+  // a B stage is two tiles of 64 K values
+  const int half_bytes = stage_rows(p.tok) * 128;
   // full barrier of B stage i at bar_b + 16 i, its free barrier 8 bytes on; the others alike.
   // A double step (128 K values) has a turn, 0 or 1 in alternation from every tile's first: two
   // A stages (one per half; full barriers by stage, freed barriers by turn), two warpgroups and
@@ -583,15 +586,19 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     int st = 0, issued = 0;
     uint32_t ph = 1;
     while (cur.valid() && ok) {
-      const int row0 = cur.row0();
+      // (What lies past the tile's rows is multiplied, and not stored, or not even that. With
+      // `tok` rows for every tile the L2 traffic was 1.8 times as much at 106 rows a tile; with
+      // several boxes of 32 rows for each tile this warp was too slow, 163 against 147 us.)
+      const int row0 = cur.row0(), boxes = (cur.row1() - row0 + kBoxRows - 1) / kBoxRows;
+      const CUtensorMap* map = &p.x[boxes - 1];
       for (int k = 0; k < steps; k += 2) {
         ok = wait_warp(bar_b + 16 * st + 8, ph, a.status, 62);
         if (!ok) break;
         const uint32_t dst = base + st * 2 * half_bytes, bar = bar_b + 16 * st;
         const bool both = k + 1 < steps;
-        arrive_tx(bar, both ? 2 * half_bytes : half_bytes, one);
-        load_tile(dst, &p.x, k * 64, row0, bar, one);
-        if (both) load_tile(dst + half_bytes, &p.x, k * 64 + 64, row0, bar, one);
+        arrive_tx(bar, (both ? 2 : 1) * boxes * kBoxRows * 128, one);
+        load_tile(dst, map, k * 64, row0, bar, one);
+        if (both) load_tile(dst + half_bytes, map, k * 64 + 64, row0, bar, one);
         ++issued;
         if (++st == p.b_stages) {
           st = 0;
@@ -703,8 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
 // The rows of x that `rows` names, one after the other; a bad index gives a row of zeros. The
 // product kernel could gather by itself, but four-row TMA loads and 16-byte cp.async both
 // brought 32 bytes a clock and SM where its MMAs take 64 (16384 rows of 2048 through 128 experts
-// of 1536x2048: 185 us with gathering inside; 13 us for this kernel, 4.9 of 6.6 TB/s copied,
-// and 134 for the product).
+// of 1536x2048: 185 us with gathering inside; 13 us for this kernel, which writes 67 MB,
+// and 130 for the product).
 __global__ void __launch_bounds__(256)
     gather_rows_kernel(const uint4* __restrict__ x, long long ldx, int x_rows,
                        const int* __restrict__ rows, uint4* __restrict__ out, int R, int per_row) {
@@ -737,9 +744,11 @@ int launch_tc_t(TcArgs& p, int grid, cudaStream_t st) {
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
   if (!make_rows_map(&p.codes, p.a.w, 1, p.a.K / 2, (long long)p.a.E * p.a.N, p.a.K / 2, 64,
-                     GATED ? 16 : 128) ||
-      !make_rows_map(&p.x, p.a.x, 2, p.a.K, p.a.x_rows, p.a.ldx * 2, 64, p.tok))
+                     GATED ? 16 : 128))
     return QKV_ECUDA;
+  for (int i = 0; i < stage_rows(p.tok) / kBoxRows; ++i)
+    if (!make_rows_map(&p.x[i], p.a.x, 2, p.a.K, p.a.x_rows, p.a.ldx * 2, 64, (i + 1) * kBoxRows))
+      return QKV_ECUDA;
   return launch(!p.gathered, matmul_tc_kernel<T, GATED>, dim3(grid), kThreads, smem, st, p);
 }
 
@@ -784,7 +793,7 @@ int launch_matmul_tc(const MatmulArgs& a, cudaStream_t st) {
   }
   const int most = std::min(a.R, p.tok);
   p.tok = (most + 15) / 16 * 16;
-  p.b_stages = std::min(kMaxBStages, kBBytes / (p.tok * 256));
+  p.b_stages = std::min(kMaxBStages, kBBytes / (stage_rows(p.tok) * 256));
   long long tiles = (long long)((a.R + p.tok - 1) / p.tok + (a.offsets ? std::min(a.E, a.R) : 0)) * p.n_tiles;
   const int grid = (int)std::min<long long>(tiles, sms);
   if (a.dtype == QKV_BF16)
