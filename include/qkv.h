@@ -256,7 +256,8 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
  * sums in fp32, one rounding at the end. bits 4, group_size 64, K a multiple of 64. With
  * QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
  * x and w 16-byte aligned, the others naturally. Non-finite x makes its own row of out
- * non-finite (inf or NaN) and no other. M = 0 does nothing.
+ * non-finite (inf or NaN) and no other; so may values above 2^114, whose sums pass
+ * the range of fp32. M = 0 does nothing.
  * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter. R rows
  * of out, E weight matrices (1 here), gathered != 0 when `rows` is given (below).
  */
