@@ -435,6 +435,12 @@ int qkv_prefill(const void* q, const void* k_new, const void* v_new, void* kw, v
 
 namespace {
 
+// Do the ranges share a byte?
+bool overlap(const void* a, long long na, const void* b, long long nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Validate and pack the shared arguments of the 4-bit weight products.
@@ -460,6 +466,9 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
     if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(out, 2) || !aligned(rows, 4) ||
         !aligned(offsets, 4))
       return fail(QKV_EALIGN, "scales, biases, out, rows and offsets must be naturally aligned");
+    const long long n_out = act == QKV_ACT_SWIGLU ? N / 2 : N;
+    if (x_rows > 0 && overlap(x, ((x_rows - 1) * ldx + K) * 2, out, R * n_out * 2))
+      return fail(QKV_EINVAL, "out overlaps x");
   }
   a = MatmulArgs{};
   a.x = x;
@@ -565,6 +574,10 @@ int qkv_expert_combine(const void* y, int R, const int* slots, const float* weig
   if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned(slots, 4) ||
       !aligned(weights, 4))
     return fail(QKV_EALIGN, "y, residual and out must be 16-byte aligned");
+  const long long bytes = (long long)T * N * 2;
+  if (overlap(y, (long long)R * N * 2, out, bytes)) return fail(QKV_EINVAL, "out overlaps y");
+  if (residual != out && overlap(residual, bytes, out, bytes))
+    return fail(QKV_EINVAL, "out overlaps the residual without being it");
   const int rc = launch_expert_combine(y, R, slots, weights, residual, out, T, k, N, dtype,
                                        static_cast<cudaStream_t>(stream));
   if (rc) return fail(rc, "expert_combine: unsupported shape");

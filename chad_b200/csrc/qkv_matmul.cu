@@ -437,7 +437,7 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   p.per = std::min(8, a.R);
   while (p.per > 0 && x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes > kDynamicBytes) --p.per;
   if (p.per < 1) return QKV_EUNSUPPORTED;
-  long long segs = (a.R + p.per - 1) / p.per;
+  long long segs = (a.R + p.per - 1ll) / p.per;
   if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
   if (segs > 65535) return QKV_EUNSUPPORTED;
   const int chunks = (a.K + kChunk - 1) / kChunk;
@@ -484,7 +484,7 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
 bool matmul_takes_tc(int R, int E, int N, int K) {
   if (!matmul_tc_fits(E, N)) return false;
   if (K > 65536) return true;  // a row of x does not fit shared memory beside the rings above
-  return R > 8ll * std::min(E, R) && (R + 7) / 8 * (long long)N > 25000;
+  return R > 8ll * std::min(E, R) && (R + 7ll) / 8 * N > 25000;
 }
 
 int launch_matmul(const MatmulArgs& a, cudaStream_t st) {

@@ -415,9 +415,9 @@ def _refuse_weights(x: torch.Tensor, w, s, b, bits: int, group_size: int, lead: 
                      f"{bits} bits, {lead} leading dimensions and group_size {group_size}")
 
 
-def _check_out(out: torch.Tensor, shape, like: torch.Tensor) -> None:
+def _check_out(out: torch.Tensor, shape, like: torch.Tensor, name: str = "out") -> None:
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {tuple(shape)} tensor of {like.dtype}")
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor of {like.dtype}")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -593,7 +593,7 @@ def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, 
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Weighted sum of every token's expert rows: (residual[t] +) sum_j weights[t,j] *
     y[slots[t,j]] for y (R, N), slots int32 and weights fp32 (T, k). Sums in fp32 in j's
-    order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual.
+    order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual, not y.
     """
     idx = y.get_device()
     if (idx < 0 or slots.get_device() != idx or weights.get_device() != idx
@@ -612,7 +612,7 @@ def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, 
     r, n = y.shape
     t, k = shape
     if residual is not None:
-        _check_out(residual, (t, n), y)
+        _check_out(residual, (t, n), y, "residual")
     if out is None:
         out = y.new_empty((t, n))
     else:

@@ -64,6 +64,13 @@ def test_route(t, e, k):
         check_route(z, k, normalize)
 
 
+@pytest.mark.parametrize("t,e,k", [(33000, 512, 2), (132000, 200, 3)])
+def test_route_of_many_tokens(t, e, k):
+    # larger blocks of tokens, whose masks pass 48 KiB of shared memory
+    gen = torch.Generator().manual_seed(t)
+    check_route(torch.randn(t, e, generator=gen).to(torch.bfloat16).cuda(), k, True)
+
+
 @pytest.mark.parametrize("t", [6, 90])
 def test_route_ties_infinities_and_nan(t):
     z = torch.zeros(t, 40)

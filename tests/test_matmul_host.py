@@ -10,7 +10,7 @@ OK, EINVAL, EUNSUP, EWS, EALIGN = (_lib.QKV_OK, _lib.QKV_EINVAL, _lib.QKV_EUNSUP
 
 
 def _matmul(lib, **over):
-    a = dict(x=16, ldx=256, w=16, s=16, b=16, out=16, M=4, N=32, K=256, bits=4, gs=64, dtype=0,
+    a = dict(x=16, ldx=256, w=16, s=16, b=16, out=1 << 20, M=4, N=32, K=256, bits=4, gs=64, dtype=0,
              act=0, ws=16, ws_bytes=1 << 30, stream=None)
     a.update(over)
     return lib.qkv_quantized_matmul(*a.values())
@@ -23,6 +23,8 @@ def _matmul(lib, **over):
     (dict(ldx=248), EINVAL), (dict(ldx=260), EALIGN), (dict(x=8), EALIGN), (dict(w=4), EALIGN),
     (dict(s=17), EALIGN), (dict(out=1), EALIGN), (dict(x=None), EINVAL), (dict(w=None), EINVAL),
     (dict(s=None), EINVAL), (dict(b=None), EINVAL), (dict(out=None), EINVAL), (dict(M=0), OK),
+    # x ends at 16 + 4 * 512, out is 4 * 64 bytes long
+    (dict(out=16), EINVAL), (dict(out=14 + 4 * 512), EINVAL), (dict(x=1024, out=770), EINVAL),
 ])
 def test_matmul_rejects_bad_arguments(over, code):
     lib = _lib.load()
@@ -32,8 +34,8 @@ def test_matmul_rejects_bad_arguments(over, code):
 
 
 def _grouped(lib, **over):
-    a = dict(x=16, ldx=256, x_rows=8, rows=None, offsets=16, w=16, s=16, b=16, out=16, R=8, E=4,
-             N=32, K=256, bits=4, gs=64, dtype=0, act=0, ws=16, ws_bytes=1 << 30, stream=None)
+    a = dict(x=16, ldx=256, x_rows=8, rows=None, offsets=16, w=16, s=16, b=16, out=1 << 20, R=8,
+             E=4, N=32, K=256, bits=4, gs=64, dtype=0, act=0, ws=16, ws_bytes=1 << 30, stream=None)
     a.update(over)
     return lib.qkv_grouped_matmul(*a.values())
 
@@ -41,7 +43,7 @@ def _grouped(lib, **over):
 @pytest.mark.parametrize("over,code", [
     (dict(offsets=None), EINVAL), (dict(R=9), EINVAL), (dict(E=0), EINVAL), (dict(bits=2), EUNSUP),
     (dict(offsets=18), EALIGN), (dict(rows=18), EALIGN), (dict(x_rows=-1), EINVAL),
-    (dict(K=100, ldx=104), EINVAL), (dict(R=0, x_rows=0), OK),
+    (dict(K=100, ldx=104), EINVAL), (dict(R=0, x_rows=0), OK), (dict(out=16), EINVAL),
 ])
 def test_grouped_rejects_bad_arguments(over, code):
     assert _grouped(_lib.load(), **over) == code
@@ -66,7 +68,7 @@ def test_route_rejects_bad_arguments(over, code):
 
 
 def _combine(lib, **over):
-    a = dict(y=16, R=32, slots=16, weights=16, residual=None, out=16, T=4, k=8, N=64, dtype=0,
+    a = dict(y=16, R=32, slots=16, weights=16, residual=None, out=1 << 20, T=4, k=8, N=64, dtype=0,
              stream=None)
     a.update(over)
     return lib.qkv_expert_combine(*a.values())
@@ -76,6 +78,8 @@ def _combine(lib, **over):
     (dict(dtype=2), EINVAL), (dict(T=-1), EINVAL), (dict(k=0), EINVAL), (dict(N=0), EINVAL),
     (dict(y=None), EINVAL), (dict(slots=None), EINVAL), (dict(out=None), EINVAL),
     (dict(out=8), EALIGN), (dict(residual=8), EALIGN), (dict(T=0), OK),
+    (dict(out=16), EINVAL), (dict(out=32 * 128), EINVAL),
+    (dict(residual=(1 << 20) + 16), EINVAL), (dict(residual=(1 << 20) - 16), EINVAL),
 ])
 def test_combine_rejects_bad_arguments(over, code):
     assert _combine(_lib.load(), **over) == code
