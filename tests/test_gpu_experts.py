@@ -233,3 +233,37 @@ def test_decode_layer_with_attention():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_two_captured_layers_at_once():
+    """Two graphs of one layer, replayed on two streams at a time on new data: no workspace is
+    shared, and the results are those of calls one by one."""
+    gen = torch.Generator().manual_seed(8)
+    e, k, f, t = 16, 256, 192, 700
+    dt = torch.bfloat16
+    layer = QuantizedExperts.from_weights((torch.randn(e, 2 * f, k, generator=gen) * k ** -0.5).to(dt).cuda(),
+                                          (torch.randn(e, k, f, generator=gen) * f ** -0.5).to(dt).cuda(), 4)
+    xs = [torch.zeros(t, k, dtype=dt, device="cuda") for _ in range(2)]
+    zs = [torch.zeros(t, e, device="cuda") for _ in range(2)]
+    layer(xs[0], zs[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, z in zip(xs, zs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(layer(x, z, residual=x))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for round_ in range(3):
+        for x, z in zip(xs, zs):
+            x.copy_(torch.randn(t, k, generator=gen))
+            z.copy_(torch.randn(t, e, generator=gen) * (round_ + 1))
+        want = [layer(x, z, residual=x) for x, z in zip(xs, zs)]
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(outs, want):
+            assert torch.equal(got, w)
