@@ -443,10 +443,13 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   const int chunks = (a.K + kChunk - 1) / kChunk;
   const size_t smem = x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes;
   const int resident = num_sms() * (smem > 104 * 1024 ? 1 : 2);
-  // CTAs per chunk of rows: as many as are resident; with experts twice that, for the bound on
-  // the chunks counts experts that may be empty (64 experts of 1536x2048 at 4 rows each 41 us
-  // with once, 35 with twice, 38 with four times as many).
-  const int ctas = (int)std::max<long long>(1, (a.offsets ? 2 : 1) * resident / segs);
+  // CTAs per chunk of rows: as many as are resident. Once more than half as many rows as experts
+  // come, half as many again: several rows then share an expert, and the bound on the chunks
+  // counts experts that are empty (1536x2048 gated, 8 rows of 128 experts 8.8 us with once, 11.1
+  // with one and a half times; 32 rows 18.4, 20.7; 64 rows 28.6, 28.2; not gated, 64 rows of 64
+  // experts 27.5, 20.8 and with twice 23.5; 256 rows 35.9, 28.9 and 31.6).
+  const int share = a.offsets && 2ll * a.R > a.E ? 3 : 2;
+  const int ctas = (int)std::max<long long>(1, share * resident / (2 * segs));
   // Warps that share K: the number whose longest warp has the least to do. A unit of a CTA costs
   // its chunks and about half a chunk more for the sums (through shared memory when shared).
   int best = 0;
