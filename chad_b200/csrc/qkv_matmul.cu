@@ -140,6 +140,17 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
   return false;
 }
 
+// How many token chunks there are, by a whole warp.
+__device__ __forceinline__ int count_chunks(const int* __restrict__ offsets, int E, int R, int per,
+                                            int lane) {
+  int n = 0;
+  for (int e = lane; e < E; e += 32) {
+    const int lo = min(max(offsets[e], 0), R), hi = min(max(offsets[e + 1], 0), R);
+    n += hi > lo ? (hi - lo + per - 1) / per : 0;
+  }
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
 constexpr int kStages = 3;                  // of one chunk, per warp
 constexpr int kCodeBytes = 16 * 128;        // 16 weight rows
 constexpr int kStageBytes = kCodeBytes + 2 * 16 * 8;  // and four scales and biases of each
@@ -154,15 +165,16 @@ struct RowsArgs {
   int wk_count;  // warps that share K
   int tiles;     // of 16 weight rows
   int per;       // rows of x per CTA (at most 8)
+  int most;      // chunks of `per` rows that the experts can have
 };
 
 // GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same outputs. SB: how a row's four
-// scales of a chunk are copied (8 bytes, 2 x 4, or one by one).
-template <typename T, bool GATED, int SB>
+// scales of a chunk are copied (8 bytes, 2 x 4, or one by one). GROUPED: with experts.
+template <typename T, bool GATED, int SB, bool GROUPED>
 __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsArgs p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][kWarps][4][32];
-  __shared__ int seg[3];
+  __shared__ int seg[3], sums_of[kWarps];
   // everything here may come from the kernel before, the weights too
   wait_for_previous();
   const MatmulArgs& a = p.a;
@@ -170,258 +182,316 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const int g = lane >> 2, t = lane & 3;
   const int wk_count = p.wk_count;
 
-  int expert = 0, row0, row1;
-  if (a.offsets) {
-    if (warp == 0) {
-      int e = 0, r0 = 0, r1 = -1;
-      find_chunk(a.offsets, a.E, a.R, p.per, blockIdx.y, lane, e, r0, r1);
-      if (lane == 0) {
-        seg[0] = e;
-        seg[1] = r0;
-        seg[2] = r1;
-      }
-    }
-    __syncthreads();
-    expert = __shfl_sync(0xffffffffu, seg[0], 0);
-    row0 = __shfl_sync(0xffffffffu, seg[1], 0);
-    row1 = __shfl_sync(0xffffffffu, seg[2], 0);
-    if (row1 < 0) return;
-  } else {
-    row0 = blockIdx.y * p.per;
-    row1 = min(row0 + p.per, a.R);
-  }
-  const int rows = row1 - row0;
   const int wk = warp % wk_count, wn = warp / wk_count, wn_count = kWarps / wk_count;
   const int n_out = GATED ? a.N / 2 : a.N;
   const int G = a.K / 64, chunks = (a.K + kChunk - 1) / kChunk, pieces = a.K / 32;
   const int units = (p.tiles + wn_count - 1) / wn_count;  // of wn_count tiles
   const uint32_t xs = smem_u32(smem);
-  const uint32_t sums = xs + (uint32_t)rows * a.K * 2;  // of each group of each row of x
-  const uint32_t zeros = sums + (uint32_t)G * 32;         // what rows past the last read
+  const uint32_t sums = xs + (uint32_t)p.per * a.K * 2;  // of each group of each row of x
+  const uint32_t zeros = sums + (uint32_t)G * 32;        // what rows past the last read
   const uint32_t ring = zeros + 128 + warp * kStages * kStageBytes;
-
-  // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
-  // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
-  auto weight_row = [&](int tile, int r) -> long long {
-    const int n = GATED ? min(tile * 8 + (r & 7), n_out - 1) + (r >> 3) * n_out
-                        : min(tile * 16 + r, n_out - 1);
-    return (long long)expert * a.N + n;
-  };
-  int ld_unit = blockIdx.x, ld_c = wk;
-  const char* src[4];  // this lane's 16 bytes of rows lane/8 + 4i of the next chunk
-  const char* ssrc;    // scales of row lane (biases of row lane - 16)
-  auto set_src = [&]() {
-    const int ld_tile = min(ld_unit * wn_count + wn, p.tiles - 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      src[i] = (const char*)a.w + weight_row(ld_tile, (lane >> 3) + 4 * i) * (a.K / 2) + ld_c * 128 +
-               (lane & 7) * 16;
-    ssrc = (const char*)(lane < 16 ? a.scales : a.biases) + weight_row(ld_tile, lane & 15) * G * 2 +
-           ld_c * 8;
-  };
-  set_src();
-  // rows lane/8 + 4i, a 512-byte step (the swizzle keeps the fragment reads apart); scales
-  const uint32_t code_to = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) & 3) << 1) << 4);
-  const uint32_t scale_to = ring + kCodeBytes + lane * 8;
-  uint32_t ld_at = 0;  // the stage's offset
-  auto load = [&]() {
-    if (ld_unit < units) {
-      if (ld_c * 8 + (lane & 7) < pieces) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cp16(code_to + ld_at + i * 512, src[i]);
+  // This CTA's units: every gridDim.x-th of its chunk of rows, or with experts an equal run of
+  // those of all their chunks, whose number only the device knows.
+  int lo, hi, id = blockIdx.y;
+  int my_lo = 0, my_hi = 0, my_n = 0, my_id = 0;  // rows, chunks and first chunk of expert threadIdx.x
+  const bool few = a.E <= kWarps * 32;            // a thread for every expert
+  if (GROUPED) {
+    if (threadIdx.x < 3) seg[threadIdx.x] = 0;
+    int all = 0;
+    if (few) {
+      if ((int)threadIdx.x < a.E) {
+        my_lo = min(max(a.offsets[threadIdx.x], 0), a.R);
+        my_hi = min(max(a.offsets[threadIdx.x + 1], 0), a.R);
+        my_n = my_hi > my_lo ? (my_hi - my_lo + p.per - 1) / p.per : 0;
       }
-      if (SB == 2) {
-        cp_small<8>(scale_to + ld_at, ssrc);
-      } else if (SB == 1) {
-        cp_small<4>(scale_to + ld_at, ssrc);
-        if (ld_c * 4 + 2 < G) cp_small<4>(scale_to + ld_at + 4, ssrc + 4);
-      } else {
+      int sum = my_n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (ld_c * 4 + j < G) {
-            const uint16_t v = __ldg((const uint16_t*)ssrc + j);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_to + ld_at + 2 * j), "h"(v) : "memory");
-          }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
       }
-      ld_c += wk_count;
-      if (ld_c >= chunks) {
-        ld_c = wk;
-        ld_unit += gridDim.x;
-        set_src();
-      } else {
+      if (lane == 31) sums_of[warp] = sum;
+      __syncthreads();
+      my_id = sum - my_n;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) src[i] += wk_count * 128;
-        ssrc += wk_count * 8;
+      for (int w = 0; w < kWarps; ++w) {
+        my_id += w < warp ? sums_of[w] : 0;
+        all += sums_of[w];
       }
+    } else {
+      if (warp == 0) {
+        const int n = count_chunks(a.offsets, a.E, a.R, p.per, lane);
+        if (lane == 0) sums_of[0] = n;
+      }
+      __syncthreads();
+      all = sums_of[0];
     }
-    ld_at = ld_at + kStageBytes == kStages * kStageBytes ? 0 : ld_at + kStageBytes;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) load();
-
-  // ---- rows of x: 128 bytes per (group, row), the 32 bytes of lane t at 32 t, values paired
-  // as the codes are, the two halves of odd rows swapped (their reads then share no bank) -----
-  for (int i = threadIdx.x; i < rows * G * 4; i += kWarps * 32) {
-    const int m = i / (G * 4), q = i - m * (G * 4);  // q = group * 4 + t
-    const int r = row0 + m;
-    const int from = a.rows ? a.rows[r] : r;
-    uint4 u = make_uint4(0, 0, 0, 0), v = u;
-    if (from >= 0 && from < a.x_rows) {
-      const uint4* at = (const uint4*)((const char*)a.x + ((long long)from * a.ldx + q * 16) * 2);
-      u = __ldg(at);
-      v = __ldg(at + 1);
-    }
-    const uint32_t to = xs + ((q >> 2) * rows + m) * 128 + (q & 3) * 32;
-    sts_v4(to + (m & 1) * 16, make_uint4(prmt(u.x, u.z, 0x5410), prmt(u.x, u.z, 0x7632),
-                                         prmt(u.y, u.w, 0x5410), prmt(u.y, u.w, 0x7632)));
-    sts_v4(to + (~m & 1) * 16, make_uint4(prmt(v.x, v.z, 0x5410), prmt(v.x, v.z, 0x7632),
-                                          prmt(v.y, v.w, 0x5410), prmt(v.y, v.w, 0x7632)));
+    // (offsets that decrease may count more chunks than there can be)
+    all = min(__shfl_sync(0xffffffffu, all, 0), p.most) * units;
+    const int each = all / (int)gridDim.x, left = all - each * (int)gridDim.x, b = blockIdx.x;
+    lo = b * each + min(b, left);
+    hi = lo + each + (b < left ? 1 : 0);
+    if (lo >= hi) return;
+    id = lo / units;
+  } else {
+    lo = 0;
+    hi = units;
   }
-  if (threadIdx.x < 8) sts_v4(zeros + threadIdx.x * 16, make_uint4(0, 0, 0, 0));
-  __syncthreads();
 
-  // one group of x as B fragments: lane (g, t) holds 16 values of row g
-  const uint32_t my_x = (g < rows ? xs + g * 128 : zeros) + t * 32, x_step = g < rows ? rows * 128 : 0;
-  auto x_frag = [&](uint32_t at, uint4 (&xv)[2]) {
-    xv[0] = lds_v4(at + (g & 1) * 16);
-    xv[1] = lds_v4(at + (~g & 1) * 16);
-  };
-  // sums of x by group, with a matrix of ones, in the unit of the codes' sums
-  for (int j = warp; j < G; j += kWarps) {
-    const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes};
-    uint4 xv[2];
-    x_frag(my_x + j * x_step, xv);
-    float d[4];
-    Codes<T>::mma0(d, ones, xv[0].x, xv[0].y);
-    Codes<T>::mma(d, ones, xv[0].z, xv[0].w);
-    Codes<T>::mma(d, ones, xv[1].x, xv[1].y);
-    Codes<T>::mma(d, ones, xv[1].z, xv[1].w);
-    if (g == 0)
-      asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + j * 32 + t * 8), "f"(d[0] * Codes<T>::kUnit),
-                   "f"(d[1] * Codes<T>::kUnit)
-                   : "memory");
-  }
-  __syncthreads();
-  uint32_t code_at[4];  // of the chunk's groups
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    code_at[j] = ring + g * 128 + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4) + (t & 1) * 8;
-  // results of a tile: lane (g, t) holds weight rows g and g + 8 for rows 2t and 2t + 1 of x
-  auto store = [&](int tile, float (&acc)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] *= 1.f / Codes<T>::kUnit;
-    const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
-    T* out = (T*)a.out;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = t * 2 + i;
-      if (r >= rows) continue;
-      T* o = out + (long long)(row0 + r) * n_out;
-      if (GATED) {
-        const float gate = acc[i], up = acc[i + 2];
-        if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
-      } else {
-        if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[i]);
-        if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[i + 2]);
-      }
-    }
-  };
-  uint32_t at = 0;  // the stage's offset
   int buf = 0;
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int tile = unit * wn_count + wn;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = wk; c < chunks; c += wk_count) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();
-      load();  // into the stage of the chunk before
-      // scales and biases of rows g and g + 8, four groups each
-      const uint32_t sat = ring + at + kCodeBytes + g * 8;
-      const uint2 sA = lds_v2(sat), sB = lds_v2(sat + 64), bA = lds_v2(sat + 128), bB = lds_v2(sat + 192);
-      uint32_t xa = my_x + c * 4 * x_step;
-      const uint32_t sum_at = sums + c * 128 + t * 8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (SB != 2 && c * 4 + j >= G) break;  // (SB 2: whole chunks)
-        const uint2 wa = lds_v2(code_at[j] + at), wb = lds_v2(code_at[j] + at + 1024);
-        uint32_t f[4][4];  // A fragments of the group's four MMAs
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u = (i & 2 ? wa.y : wa.x) >> (8 * (i & 1));
-          const uint32_t v = (i & 2 ? wb.y : wb.x) >> (8 * (i & 1));
-          f[i][0] = and_or(u, 0x000f000fu, Codes<T>::kMagic);
-          f[i][1] = and_or(v, 0x000f000fu, Codes<T>::kMagic);
-          f[i][2] = and_or(u >> 4, 0x000f000fu, Codes<T>::kMagic);
-          f[i][3] = and_or(v >> 4, 0x000f000fu, Codes<T>::kMagic);
+  for (int first = GROUPED ? id * units : 0; first < hi; first += units, ++id) {
+    const int unit0 = GROUPED ? max(lo - first, 0) : blockIdx.x;
+    const int unit1 = GROUPED ? min(hi - first, units) : units;
+    const int step = GROUPED ? 1 : gridDim.x;
+    int expert = 0, row0, row1;
+    if (GROUPED) {
+      if (few) {
+        if (id >= my_id && id < my_id + my_n) {
+          seg[0] = threadIdx.x;
+          seg[1] = my_lo + (id - my_id) * p.per;
+          seg[2] = min(my_lo + (id - my_id + 1) * p.per, my_hi);
         }
-        const uint32_t s0 = j < 2 ? sA.x : sA.y, s1 = j < 2 ? sB.x : sB.y;
-        const uint32_t b0 = j < 2 ? bA.x : bA.y, b1 = j < 2 ? bB.x : bB.y;
-        const int sh = (j & 1) * 16;
-        const float q0 = Elem<T>::bits_to_f32((uint16_t)(s0 >> sh));
-        const float q1 = Elem<T>::bits_to_f32((uint16_t)(s1 >> sh));
-        const float o0 = Codes<T>::bias(q0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
-        const float o1 = Codes<T>::bias(q1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
-        uint4 xv[2];
-        x_frag(xa, xv);
-        xa += x_step;
-        float d[4];
-        Codes<T>::mma0(d, f[0], xv[0].x, xv[0].y);
-        Codes<T>::mma(d, f[1], xv[0].z, xv[0].w);
-        Codes<T>::mma(d, f[2], xv[1].x, xv[1].y);
-        Codes<T>::mma(d, f[3], xv[1].z, xv[1].w);
-        const uint2 sx = lds_v2(sum_at + j * 32);
-        const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
-        acc[0] = fmaf(q0, d[0], fmaf(o0, sx0, acc[0]));
-        acc[1] = fmaf(q0, d[1], fmaf(o0, sx1, acc[1]));
-        acc[2] = fmaf(q1, d[2], fmaf(o1, sx0, acc[2]));
-        acc[3] = fmaf(q1, d[3], fmaf(o1, sx1, acc[3]));
+      } else if (warp == 0) {
+        int e = 0, r0 = 0, r1 = 0;
+        find_chunk(a.offsets, a.E, a.R, p.per, id, lane, e, r0, r1);
+        if (lane == 0) {
+          seg[0] = e;
+          seg[1] = r0;
+          seg[2] = r1;
+        }
       }
-      at = at + kStageBytes == kStages * kStageBytes ? 0 : at + kStageBytes;
+      __syncthreads();  // (and no warp reads the rows of the chunk before)
+      expert = __shfl_sync(0xffffffffu, seg[0], 0);
+      row0 = __shfl_sync(0xffffffffu, seg[1], 0);
+      row1 = __shfl_sync(0xffffffffu, seg[2], 0);
+    } else {
+      row0 = id * p.per;
+      row1 = min(row0 + p.per, a.R);
     }
+    const int rows = row1 - row0;
 
-    if (wk_count > 1) {
-      // (two buffers: the reader of this unit's passes the next unit's barrier before anyone
-      // writes here again)
-      if (wk) {
+    // ---- the warp's stream of chunks: its tile of every unit, chunks wk, wk + wk_count, ... ----
+    // weight row of row r of a tile (clamped into the matrix; what is past it is not stored)
+    auto weight_row = [&](int tile, int r) -> long long {
+      const int n = GATED ? min(tile * 8 + (r & 7), n_out - 1) + (r >> 3) * n_out
+                          : min(tile * 16 + r, n_out - 1);
+      return (long long)expert * a.N + n;
+    };
+    int ld_unit = unit0, ld_c = wk;
+    const char* src[4];  // this lane's 16 bytes of rows lane/8 + 4i of the next chunk
+    const char* ssrc;    // scales of row lane (biases of row lane - 16)
+    auto set_src = [&]() {
+      const int ld_tile = min(ld_unit * wn_count + wn, p.tiles - 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[buf][warp][i][lane] = acc[i];
-      }
-      named_bar_sync(1 + wn, wk_count * 32);
-      if (!wk) {
-        for (int o = 1; o < wk_count; ++o)
+      for (int i = 0; i < 4; ++i)
+        src[i] = (const char*)a.w + weight_row(ld_tile, (lane >> 3) + 4 * i) * (a.K / 2) + ld_c * 128 +
+                 (lane & 7) * 16;
+      ssrc = (const char*)(lane < 16 ? a.scales : a.biases) + weight_row(ld_tile, lane & 15) * G * 2 +
+             ld_c * 8;
+    };
+    set_src();
+    // rows lane/8 + 4i, a 512-byte step (the swizzle keeps the fragment reads apart); scales
+    const uint32_t code_to = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) & 3) << 1) << 4);
+    const uint32_t scale_to = ring + kCodeBytes + lane * 8;
+    uint32_t ld_at = 0;  // the stage's offset
+    auto load = [&]() {
+      if (ld_unit < unit1) {
+        if (ld_c * 8 + (lane & 7) < pieces) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] += red[buf][warp + o][i][lane];
+          for (int i = 0; i < 4; ++i) cp16(code_to + ld_at + i * 512, src[i]);
+        }
+        if (SB == 2) {
+          cp_small<8>(scale_to + ld_at, ssrc);
+        } else if (SB == 1) {
+          cp_small<4>(scale_to + ld_at, ssrc);
+          if (ld_c * 4 + 2 < G) cp_small<4>(scale_to + ld_at + 4, ssrc + 4);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (ld_c * 4 + j < G) {
+              const uint16_t v = __ldg((const uint16_t*)ssrc + j);
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(scale_to + ld_at + 2 * j), "h"(v) : "memory");
+            }
+        }
+        ld_c += wk_count;
+        if (ld_c >= chunks) {
+          ld_c = wk;
+          ld_unit += step;
+          set_src();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) src[i] += wk_count * 128;
+          ssrc += wk_count * 8;
+        }
       }
-      buf ^= 1;
+      ld_at = ld_at + kStageBytes == kStages * kStageBytes ? 0 : ld_at + kStageBytes;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) load();
+
+    // ---- rows of x: 128 bytes per (group, row), the 32 bytes of lane t at 32 t, values paired
+    // as the codes are, the two halves of odd rows swapped (their reads then share no bank) -----
+    for (int i = threadIdx.x; i < rows * G * 4; i += kWarps * 32) {
+      const int m = i / (G * 4), q = i - m * (G * 4);  // q = group * 4 + t
+      const int r = row0 + m;
+      const int from = a.rows ? a.rows[r] : r;
+      uint4 u = make_uint4(0, 0, 0, 0), v = u;
+      if (from >= 0 && from < a.x_rows) {
+        const uint4* at = (const uint4*)((const char*)a.x + ((long long)from * a.ldx + q * 16) * 2);
+        u = __ldg(at);
+        v = __ldg(at + 1);
+      }
+      const uint32_t to = xs + ((q >> 2) * rows + m) * 128 + (q & 3) * 32;
+      sts_v4(to + (m & 1) * 16, make_uint4(prmt(u.x, u.z, 0x5410), prmt(u.x, u.z, 0x7632),
+                                           prmt(u.y, u.w, 0x5410), prmt(u.y, u.w, 0x7632)));
+      sts_v4(to + (~m & 1) * 16, make_uint4(prmt(v.x, v.z, 0x5410), prmt(v.x, v.z, 0x7632),
+                                            prmt(v.y, v.w, 0x5410), prmt(v.y, v.w, 0x7632)));
     }
-    if (wk == 0 && tile < p.tiles) store(tile, acc);
+    if (threadIdx.x < 8) sts_v4(zeros + threadIdx.x * 16, make_uint4(0, 0, 0, 0));
+    __syncthreads();
+
+    // one group of x as B fragments: lane (g, t) holds 16 values of row g
+    const uint32_t my_x = (g < rows ? xs + g * 128 : zeros) + t * 32, x_step = g < rows ? rows * 128 : 0;
+    auto x_frag = [&](uint32_t at, uint4 (&xv)[2]) {
+      xv[0] = lds_v4(at + (g & 1) * 16);
+      xv[1] = lds_v4(at + (~g & 1) * 16);
+    };
+    // sums of x by group, with a matrix of ones, in the unit of the codes' sums
+    for (int j = warp; j < G; j += kWarps) {
+      const uint32_t ones[4] = {Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes, Codes<T>::kOnes};
+      uint4 xv[2];
+      x_frag(my_x + j * x_step, xv);
+      float d[4];
+      Codes<T>::mma0(d, ones, xv[0].x, xv[0].y);
+      Codes<T>::mma(d, ones, xv[0].z, xv[0].w);
+      Codes<T>::mma(d, ones, xv[1].x, xv[1].y);
+      Codes<T>::mma(d, ones, xv[1].z, xv[1].w);
+      if (g == 0)
+        asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(sums + j * 32 + t * 8), "f"(d[0] * Codes<T>::kUnit),
+                     "f"(d[1] * Codes<T>::kUnit)
+                     : "memory");
+    }
+    __syncthreads();
+    uint32_t code_at[4];  // of the chunk's groups
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      code_at[j] = ring + g * 128 + (((2 * j + (t >> 1)) ^ (g & 3) << 1) << 4) + (t & 1) * 8;
+    // results of a tile: lane (g, t) holds weight rows g and g + 8 for rows 2t and 2t + 1 of x
+    auto store = [&](int tile, float (&acc)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] *= 1.f / Codes<T>::kUnit;
+      const int nA = GATED ? tile * 8 + g : tile * 16 + g, nB = GATED ? nA : nA + 8;
+      T* out = (T*)a.out;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = t * 2 + i;
+        if (r >= rows) continue;
+        T* o = out + (long long)(row0 + r) * n_out;
+        if (GATED) {
+          const float gate = acc[i], up = acc[i + 2];
+          if (nA < n_out) o[nA] = Elem<T>::from_f32(gate / (1.f + expf(-gate)) * up);
+        } else {
+          if (nA < n_out) o[nA] = Elem<T>::from_f32(acc[i]);
+          if (nB < n_out) o[nB] = Elem<T>::from_f32(acc[i + 2]);
+        }
+      }
+    };
+    uint32_t at = 0;  // the stage's offset
+    for (int unit = unit0; unit < unit1; unit += step) {
+      const int tile = unit * wn_count + wn;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int c = wk; c < chunks; c += wk_count) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        load();  // into the stage of the chunk before
+        // scales and biases of rows g and g + 8, four groups each
+        const uint32_t sat = ring + at + kCodeBytes + g * 8;
+        const uint2 sA = lds_v2(sat), sB = lds_v2(sat + 64), bA = lds_v2(sat + 128), bB = lds_v2(sat + 192);
+        uint32_t xa = my_x + c * 4 * x_step;
+        const uint32_t sum_at = sums + c * 128 + t * 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (SB != 2 && c * 4 + j >= G) break;  // (SB 2: whole chunks)
+          const uint2 wa = lds_v2(code_at[j] + at), wb = lds_v2(code_at[j] + at + 1024);
+          uint32_t f[4][4];  // A fragments of the group's four MMAs
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = (i & 2 ? wa.y : wa.x) >> (8 * (i & 1));
+            const uint32_t v = (i & 2 ? wb.y : wb.x) >> (8 * (i & 1));
+            f[i][0] = and_or(u, 0x000f000fu, Codes<T>::kMagic);
+            f[i][1] = and_or(v, 0x000f000fu, Codes<T>::kMagic);
+            f[i][2] = and_or(u >> 4, 0x000f000fu, Codes<T>::kMagic);
+            f[i][3] = and_or(v >> 4, 0x000f000fu, Codes<T>::kMagic);
+          }
+          const uint32_t s0 = j < 2 ? sA.x : sA.y, s1 = j < 2 ? sB.x : sB.y;
+          const uint32_t b0 = j < 2 ? bA.x : bA.y, b1 = j < 2 ? bB.x : bB.y;
+          const int sh = (j & 1) * 16;
+          const float q0 = Elem<T>::bits_to_f32((uint16_t)(s0 >> sh));
+          const float q1 = Elem<T>::bits_to_f32((uint16_t)(s1 >> sh));
+          const float o0 = Codes<T>::bias(q0, Elem<T>::bits_to_f32((uint16_t)(b0 >> sh)));
+          const float o1 = Codes<T>::bias(q1, Elem<T>::bits_to_f32((uint16_t)(b1 >> sh)));
+          uint4 xv[2];
+          x_frag(xa, xv);
+          xa += x_step;
+          float d[4];
+          Codes<T>::mma0(d, f[0], xv[0].x, xv[0].y);
+          Codes<T>::mma(d, f[1], xv[0].z, xv[0].w);
+          Codes<T>::mma(d, f[2], xv[1].x, xv[1].y);
+          Codes<T>::mma(d, f[3], xv[1].z, xv[1].w);
+          const uint2 sx = lds_v2(sum_at + j * 32);
+          const float sx0 = __uint_as_float(sx.x), sx1 = __uint_as_float(sx.y);
+          acc[0] = fmaf(q0, d[0], fmaf(o0, sx0, acc[0]));
+          acc[1] = fmaf(q0, d[1], fmaf(o0, sx1, acc[1]));
+          acc[2] = fmaf(q1, d[2], fmaf(o1, sx0, acc[2]));
+          acc[3] = fmaf(q1, d[3], fmaf(o1, sx1, acc[3]));
+        }
+        at = at + kStageBytes == kStages * kStageBytes ? 0 : at + kStageBytes;
+      }
+
+      if (wk_count > 1) {
+        // (two buffers: the reader of this unit's passes the next unit's barrier before anyone
+        // writes here again)
+        if (wk) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) red[buf][warp][i][lane] = acc[i];
+        }
+        named_bar_sync(1 + wn, wk_count * 32);
+        if (!wk) {
+          for (int o = 1; o < wk_count; ++o)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += red[buf][warp + o][i][lane];
+        }
+        buf ^= 1;
+      }
+      if (wk == 0 && tile < p.tiles) store(tile, acc);
+    }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, bool GATED, int SB>
+template <typename T, bool GATED, int SB, bool GROUPED>
 int launch_rows_s(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};  // devices whose shared memory bound is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ECUDA;
   if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
-    if (cudaFuncSetAttribute(matmul_rows_kernel<T, GATED, SB>,
+    if (cudaFuncSetAttribute(matmul_rows_kernel<T, GATED, SB, GROUPED>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kDynamicBytes) != cudaSuccess)
       return QKV_ECUDA;
     if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
   }
-  return launch(true, matmul_rows_kernel<T, GATED, SB>, grid, kWarps * 32, smem, st, p);
+  return launch(true, matmul_rows_kernel<T, GATED, SB, GROUPED>, grid, kWarps * 32, smem, st, p);
 }
 
-template <typename T, bool GATED>
+template <typename T, bool GATED, bool GROUPED>
 int launch_rows_g(const RowsArgs& p, dim3 grid, size_t smem, cudaStream_t st) {
   const int groups = p.a.K / 64;
   const uintptr_t at = (uintptr_t)p.a.scales | (uintptr_t)p.a.biases;
-  if (groups % 4 == 0 && at % 8 == 0) return launch_rows_s<T, GATED, 2>(p, grid, smem, st);
-  if (groups % 2 == 0 && at % 4 == 0) return launch_rows_s<T, GATED, 1>(p, grid, smem, st);
-  return launch_rows_s<T, GATED, 0>(p, grid, smem, st);
+  if (groups % 4 == 0 && at % 8 == 0) return launch_rows_s<T, GATED, 2, GROUPED>(p, grid, smem, st);
+  if (groups % 2 == 0 && at % 4 == 0) return launch_rows_s<T, GATED, 1, GROUPED>(p, grid, smem, st);
+  return launch_rows_s<T, GATED, 0, GROUPED>(p, grid, smem, st);
 }
 
 template <typename T>
@@ -439,24 +509,22 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   if (p.per < 1) return QKV_EUNSUPPORTED;
   long long segs = (a.R + p.per - 1ll) / p.per;
   if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
-  if (segs > 65535) return QKV_EUNSUPPORTED;
+  if (!a.offsets && segs > 65535) return QKV_EUNSUPPORTED;
   const int chunks = (a.K + kChunk - 1) / kChunk;
   const size_t smem = x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes;
   const int resident = num_sms() * (smem > 104 * 1024 ? 1 : 2);
-  // CTAs per chunk of rows: as many as are resident. Once more than half as many rows as experts
-  // come, half as many again: several rows then share an expert, and the bound on the chunks
-  // counts experts that are empty (1536x2048 gated, 8 rows of 128 experts 8.8 us with once, 11.1
-  // with one and a half times; 32 rows 18.4, 20.7; 64 rows 28.6, 28.2; not gated, 64 rows of 64
-  // experts 27.5, 20.8 and with twice 23.5; 256 rows 35.9, 28.9 and 31.6).
-  const int share = a.offsets && 2ll * a.R > a.E ? 3 : 2;
-  const int ctas = (int)std::max<long long>(1, share * resident / (2 * segs));
   // Warps that share K: the number whose longest warp has the least to do. A unit of a CTA costs
   // its chunks and about half a chunk more for the sums (through shared memory when shared).
+  // With experts that is a guess: the bound on their chunks counts empty experts too, unless
+  // there are few rows.
+  const long long guess = !a.offsets || 2ll * a.R <= a.E ? segs : (2 * segs + 2) / 3;
   int best = 0;
   long long best_cost = 0;
   for (int wk = 1; wk <= kWarps && wk <= chunks; wk *= 2) {
     const int units = (p.tiles + kWarps / wk - 1) / (kWarps / wk);
-    const long long rounds = (units + ctas - 1) / ctas;
+    const long long ctas = std::max(1ll, resident / segs);
+    const long long rounds = a.offsets ? (guess * units + resident - 1) / resident
+                                       : (units + ctas - 1) / ctas;
     const long long cost = rounds * (4 * ((chunks + wk - 1) / wk) + (wk > 1 ? 2 : 1));
     if (!best || cost < best_cost) {
       best = wk;
@@ -465,9 +533,17 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   }
   p.wk_count = best;
   const int units = (p.tiles + kWarps / best - 1) / (kWarps / best);
-  const dim3 grid((unsigned)std::min(units, ctas), (unsigned)segs);
-  return gated ? launch_rows_g<T, true>(p, grid, smem, st)
-               : launch_rows_g<T, false>(p, grid, smem, st);
+  if (a.offsets && segs * units > 0x7fffffffll) return QKV_EUNSUPPORTED;
+  p.most = (int)std::min<long long>(segs, 0x7fffffff);
+  const dim3 grid =
+      a.offsets ? dim3((unsigned)std::min<long long>(resident, segs * units))
+                : dim3((unsigned)std::min<long long>(units, std::max(1ll, resident / segs)),
+                       (unsigned)segs);
+  if (a.offsets)
+    return gated ? launch_rows_g<T, true, true>(p, grid, smem, st)
+                 : launch_rows_g<T, false, true>(p, grid, smem, st);
+  return gated ? launch_rows_g<T, true, false>(p, grid, smem, st)
+               : launch_rows_g<T, false, false>(p, grid, smem, st);
 }
 
 }  // namespace
