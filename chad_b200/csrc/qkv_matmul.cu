@@ -554,16 +554,19 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
 }
 
 // Few rows go to the kernel above, which reads the weights once per eight rows; the tcgen05
-// kernel reads them once, but dequantizes no more than 2.3 TB/s of them and takes 12 to 18 us at
-// the least. One pass over the weights is always better with the first (12288x2048 at 8 rows
-// 9.0 against 12.8 us); more passes as long as they are short (16 rows 12.1 against 12.8, 24
-// rows 13.8 against 13.2; 5120x2048 at 32 rows 11.4 against 13.0, at 48 13.6 against 13.3;
-// 2048x4096 at 64 rows 15.4 against 19.3, at 96 21.2 against 20.5; 64 experts of 1536x2048 at 8
-// rows each 47.7 against 49.7, at 12 60.8 against 50.4).
+// kernel reads them once, but takes 6 us and 2.6 for every 1024 of K and round of 128 x 192 tiles
+// over the SMs, the other 4 and 1 for every 8 million weights of a pass (both measured, to 15%).
+// us of this and of that kernel at 16, 32, 64 and 96 rows: 2048x4096 6.8 9.2 13.7 18.6, 16.7 17.0
+// 17.7 18.8; 5120x2048 8.3 10.9 16.0 19.9, 11.4 11.6 12.1 12.8; 12288x2048 11.4 16.9 27.3 34.9,
+// 11.9 12.1 12.8 13.5; 2048x16384 25.7 42.4 79.1 105, 49.4 50.2 51.8 54.7. Experts' rows are
+// no more than 8 each up to R = 8 E, whatever the sizes then: 4, 8 and 12 rows for each of 64
+// experts of 1536x2048 30.9 41.8 53.2, 39.1 44.9 45.7; 8 and 10 for each of 128 73.1 85.0, 75.0 77.8.
 bool matmul_takes_tc(int R, int E, int N, int K) {
   if (!matmul_tc_fits(E, N)) return false;
   if (K > 65536) return true;  // a row of x does not fit shared memory beside the rings above
-  return R > 8ll * std::min(E, R) && (R + 7ll) / 8 * N > 25000;
+  if (R <= 8ll * std::min(E, R)) return false;
+  const long long passes = (R + 7ll) / 8, tiles = (N + 127ll) / 128 * ((R + 191ll) / 192);
+  return passes * N > 16000000 / K + 20000 * ((tiles + 147) / 148);
 }
 
 int launch_matmul(const MatmulArgs& a, cudaStream_t st) {
