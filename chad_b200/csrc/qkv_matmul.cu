@@ -533,7 +533,7 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   }
   p.wk_count = best;
   const int units = (p.tiles + kWarps / best - 1) / (kWarps / best);
-  if (a.offsets && segs * units > 0x7fffffffll) return QKV_EUNSUPPORTED;
+  if (a.offsets && segs * units > 1ll << 30) return QKV_EUNSUPPORTED;
   p.most = (int)std::min<long long>(segs, 0x7fffffff);
   const dim3 grid =
       a.offsets ? dim3((unsigned)std::min<long long>(resident, segs * units))
@@ -564,6 +564,7 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
 bool matmul_takes_tc(int R, int E, int N, int K) {
   if (!matmul_tc_fits(E, N)) return false;
   if (K > 65536) return true;  // a row of x does not fit shared memory beside the rings above
+  if (R > 65528) return true;  // the kernel above has one grid row for every eight at most
   if (R <= 8ll * std::min(E, R)) return false;
   const long long passes = (R + 7ll) / 8, tiles = (N + 127ll) / 128 * ((R + 191ll) / 192);
   return passes * N > 16000000 / K + 20000 * ((tiles + 147) / 148);

@@ -255,8 +255,8 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
  * scales and biases (N, K/64), out (M, N); x, scales, biases and out in `dtype` (bf16 or f16),
  * sums in fp32, one rounding at the end. bits 4, group_size 64, K a multiple of 64. With
  * QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
- * x and w 16-byte aligned, the others naturally; out apart from x. Non-finite x makes its own row of out
- * non-finite (inf or NaN) and no other; so may values above 2^114, whose sums pass
+ * x and w 16-byte aligned, the others naturally; out apart from x. Non-finite x makes its own
+ * row of out non-finite (inf or NaN) and no other; so may values above 2^114, whose sums pass
  * the range of fp32. M = 0 does nothing.
  * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter. R rows
  * of out, E weight matrices (1 here), gathered != 0 when `rows` is given (below).
@@ -275,8 +275,9 @@ int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void
  *
  * w (E, N, K/8), scales and biases (E, N, K/64), offsets device int32[E+1] (ascending, within
  * [0, R]), rows device int32[R] or NULL. Rows of out outside [offsets[0], offsets[E]) are not
- * written. Offsets outside [0, R] are clamped and a decreasing pair is an empty expert; an
- * entry of rows outside [0, x_rows) reads a row of zeros.
+ * written. Offsets outside [0, R] are clamped and a decreasing pair is an empty expert (rows
+ * that it leaves to two experts hold either's result); an entry of rows outside [0, x_rows)
+ * reads a row of zeros.
  */
 int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows,
                        const int* offsets, const void* w, const void* scales,

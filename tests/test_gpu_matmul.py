@@ -231,6 +231,32 @@ def test_grouped(counts, n, k, act, dtype, gather):
         at += c
 
 
+@pytest.mark.parametrize("counts", [[1, 0, 2] * 100, [0] * 699 + [11], [21, 0, 0, 9] * 275,
+                                    [3] * 1025, [40, 0, 0, 0] * 260])
+def test_more_experts_than_threads(counts):
+    # more than a block has threads, and more than the kernel for many rows takes
+    gen = torch.Generator().manual_seed(len(counts))
+    wq = make_weights(gen, (len(counts), 24), 128, torch.bfloat16)
+    offsets = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    x = torch.randn(sum(counts), 128, generator=gen).bfloat16().cuda()
+    got = ops.grouped_quantized_matmul(x, wq, offsets)
+    at = 0
+    for i, c in enumerate(counts):
+        if c:
+            want, err = reference(x[at:at + c], [t[i] for t in wq], None, torch.bfloat16)
+            check(got[at:at + c], want, err, f"expert {i} of {len(counts)}")
+        at += c
+
+
+@pytest.mark.parametrize("m,n", [(8193, 1), (65528, 3), (65529, 3), (70000, 16), (600000, 1)])
+def test_many_rows_through_few_weights(m, n):
+    gen = torch.Generator().manual_seed(m)
+    wq = make_weights(gen, (n,), 64, torch.float16)
+    x = torch.randn(m, 64, generator=gen).half().cuda()
+    want, err = reference(x, wq, None, torch.float16)
+    check(ops.quantized_matmul(x, wq), want, err, f"{m} rows, {n} weights")
+
+
 @pytest.mark.parametrize("counts", [[3, 0, 5], [90, 0, 100]])
 def test_rows_outside_the_offsets_are_left_alone(counts):
     gen = torch.Generator().manual_seed(11)
@@ -366,3 +392,134 @@ def test_weights_past_32_bit_offsets():
         got = ops.grouped_quantized_matmul(x, (w, s, b), off)
         want, err = reference(x, (lw, ls, lb), None, torch.bfloat16)
         check(got, want, err, f"last of {e} experts, {r} rows")
+
+
+# ---------------------------------------------------------------------------------------
+# the kernel for many rows, at sizes that are sure to reach it
+# ---------------------------------------------------------------------------------------
+
+def takes_many(r, e, n, k):
+    """Does the library take these rows to the kernel that gathers into a workspace?"""
+    return _lib.load().qkv_matmul_workspace_size(r, e, n, k, 1) > 0
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (300, 1000, 1088), (1000, 514, 832), (2000, 302, 320), (4000, 600, 64), (5000, 258, 128),
+    (9000, 34, 2112), (193, 2000, 704), (33, 20000, 960), (17, 40002, 1984), (200, 1301, 4096),
+    (384, 900, 1984), (64, 8190, 1024), (1537, 1026, 576), (100, 16384, 192),
+])
+@pytest.mark.parametrize("act", [None, "swiglu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_matmul_of_many_rows(m, n, k, act, dtype):
+    n += n % 2 if act else 0
+    assert takes_many(m, 1, n, k)
+    gen = torch.Generator().manual_seed(m * 7 + n)
+    dt = DT[dtype]
+    wq = make_weights(gen, (n,), k, dt)
+    x = torch.randn(m, k, generator=gen).to(dt).cuda()
+    want, err = reference(x, wq, act, dt)
+    got = ops.quantized_matmul(x, wq, activation=act)
+    check(got, want, err, f"{m} x {k} through {n} {act} {dtype}")
+    # a strided view, results in place and nothing past them, the same once more
+    big = torch.randn(m, k + 72, generator=gen).to(dt).cuda()
+    big[:, 40:40 + k] = x
+    pool = torch.full((m + 2, got.shape[1]), 7.0, dtype=dt, device="cuda")
+    ops.quantized_matmul(big[:, 40:40 + k], wq, activation=act, out=pool[1:m + 1])
+    assert torch.equal(pool[1:m + 1], got)
+    assert bool((pool[0] == 7).all()) and bool((pool[-1] == 7).all())
+
+
+@pytest.mark.parametrize("counts,n,k", [
+    ([200, 1, 0, 300, 17], 700, 1088), ([129, 256, 127], 640, 1024), ([64] * 8, 1100, 704),
+    ([500, 0, 0, 1], 702, 960), ([17] * 33, 1026, 320), ([2] * 10 + [900], 500, 576),
+    ([0, 0, 1000], 514, 512), ([193, 385, 31, 33, 0, 16, 15], 900, 640),
+    ([3, 90, 0, 40, 250, 8, 1, 1, 60, 11], 4098, 192), ([70] * 60, 130, 1408),
+])
+@pytest.mark.parametrize("act", [None, "swiglu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_grouped_of_many_rows(counts, n, k, act, dtype, gather):
+    assert takes_many(sum(counts), len(counts), n, k)
+    test_grouped(counts, n, k, act, dtype, gather)
+
+
+def test_many_rows_that_are_not_finite_or_not_there():
+    gen = torch.Generator().manual_seed(18)
+    r, n, k = 640, 900, 640
+    assert takes_many(r, 3, n, k) and takes_many(r, 1, n, k)
+    wq = make_weights(gen, (3, n), k, torch.bfloat16)
+    one = tuple(t[0] for t in wq)
+    x = torch.randn(r, k, generator=gen).bfloat16().cuda()
+    want = ops.quantized_matmul(x, one)
+    y = x.clone()
+    y[1, 17], y[200, 600] = float("inf"), float("nan")
+    got = ops.quantized_matmul(y, one)
+    keep = torch.tensor([i for i in range(r) if i not in (1, 200)], device="cuda")
+    assert torch.equal(got[keep], want[keep])
+    assert not bool(torch.isfinite(got[[1, 200]]).any())
+    # rows before, between and after the experts' are left alone
+    off = torch.tensor([2, 250, 250, 600], dtype=torch.int32, device="cuda")
+    out = torch.full((r, n), 9.0, dtype=torch.bfloat16, device="cuda")
+    ops.grouped_quantized_matmul(x, wq, off, out=out)
+    assert bool((out[:2] == 9).all()) and bool((out[600:] == 9).all())
+    for i, (a, b) in ((0, (2, 250)), (2, (250, 600))):
+        ref, err = reference(x[a:b], [t[i] for t in wq], None, torch.bfloat16)
+        check(out[a:b], ref, err, f"expert {i}")
+    # bad offsets and rows stay inside
+    rows = torch.arange(r, dtype=torch.int32)
+    rows[1], rows[300] = -1, r
+    off = torch.tensor([-5, 320, 320, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    out = ops.grouped_quantized_matmul(x, wq, off, rows=rows.cuda())
+    src = x.clone()
+    src[1] = src[300] = 0
+    for i, (a, b) in ((0, (0, 320)), (2, (320, r))):
+        ref, err = reference(src[a:b], [t[i] for t in wq], None, torch.bfloat16)
+        check(out[a:b], ref, err, f"expert {i}")
+    out = torch.full((r, n), 9.0, dtype=torch.bfloat16, device="cuda")
+    ops.grouped_quantized_matmul(x, wq, torch.tensor([r, 1, 1, 1], dtype=torch.int32, device="cuda"), out=out)
+    assert bool((out == 9).all())
+
+
+def test_many_rows_on_two_streams_and_in_graphs():
+    gen = torch.Generator().manual_seed(19)
+    r, e, n, k = 700, 4, 1000, 512
+    assert takes_many(r, e, n, k) and takes_many(r, 1, n, k)
+    wq = make_weights(gen, (e, n), k, torch.bfloat16)
+    one = tuple(t[0] for t in wq)
+    xs = [torch.randn(r, k, generator=gen).bfloat16().cuda() for _ in range(2)]
+    rows = torch.randint(0, r, (r,), generator=gen, dtype=torch.int32).cuda()
+    off = torch.tensor([0, 100, 100, 333, r], dtype=torch.int32, device="cuda")
+
+    def calls(x):
+        return (ops.quantized_matmul(x, one, activation="swiglu"),
+                ops.grouped_quantized_matmul(x, wq, off, rows=rows))
+
+    want = [calls(x) for x in xs]
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in xs], [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(calls(x))
+        graphs.append(graph)
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls(xs[i]))
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in (*got[i], outs[i]):
+            assert torch.equal(pair[0], want[i][0]) and torch.equal(pair[1], want[i][1])
+    # new data; the pair 200, 100 decreases, and rows 100 to 199 are the first and third expert's
+    xs[0].copy_(xs[1])
+    off[1] = 200
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0][0], calls(xs[0])[0])
+    by = [ops.quantized_matmul(xs[0][rows.long()], tuple(t[i] for t in wq)) for i in (0, 2, 3)]
+    got = outs[0][1]
+    assert torch.equal(got[:100], by[0][:100])
+    assert bool(((got == by[0]) | (got == by[1]))[100:200].all())
+    assert torch.equal(got[200:333], by[1][200:333]) and torch.equal(got[333:], by[2][333:])
