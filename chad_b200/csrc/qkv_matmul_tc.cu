@@ -27,11 +27,11 @@
 // rounding included) against its 1.7e-3, of a gated product by 2.7e-3 against 1.7e-3; in f16 by
 // 2.8e-4 and 3.4e-4 against 2.1e-4. Weights in two terms would double the MMAs and the stores.
 //
-// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 143 us: the tensor pipe is
+// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 141 us: the tensor pipe is
 // busy 47% of the time, the ALU pipe with dequantizing 52% (its warps wait for
 // freed A stages about as often as the MMAs wait for full ones), HBM at 1.8 TB/s. 2048 rows through
-// 5120x2048: 33.6 us, 1280 TFLOP/s, tensor pipe 62 to 76%. Run without a pause both are at the
-// card's power limit (1550 MHz): 168 and 40 us.
+// 5120x2048: 32.7 us, 1310 TFLOP/s, tensor pipe 62 to 76%. Run without a pause both are at the
+// card's power limit (1540 MHz): 160 and 39 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -145,8 +145,16 @@ __device__ __forceinline__ uint32_t elect_one() {
   return p;
 }
 
-// Barrier waits by shared address: one poll inline, a wait that lasts out of line, bounded as
-// every wait of the library. (try_wait without a time limit: with one it is a loop of its own,
+// A value that all lanes have, in a uniform register. The loops that issue MMAs and copies count
+// to such values and call no function (which would not preserve the registers): their operands
+// then stay in uniform registers, instead of being moved there for every instruction (16384
+// expert rows 146 us with loops that the compiler takes for divergent, 141 so).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __reduce_max_sync(0xffffffffu, v);
+}
+
+// Barrier waits by shared address: one poll inline, a wait that lasts out of line (but for the
+// warps that issue), bounded as every wait of the library. (try_wait without a time limit: with one it is a loop of its own,
 // which took a third of all instructions; sleeping between the polls gained nothing.)
 __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -187,13 +195,27 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* st
   if (__all_sync(0xffffffffu, poll(bar, parity))) return true;
   return __all_sync(0xffffffffu, wait_long(bar, parity, status, where));
 }
+// the same without a call
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, int* status, int where) {
+  unsigned long long t0 = 0;
+  for (uint32_t i = 1; !__all_sync(0xffffffffu, poll(bar, parity)); ++i) {
+    if (i & 255) continue;
+    const unsigned long long t = global_ns();
+    if (!t0) t0 = t;
+    if (__any_sync(0xffffffffu, t - t0 > kSpinNanos || i >= kSpinLimit)) {
+      flag_device_error(status, where);
+      return false;
+    }
+  }
+  return true;
+}
 // three barriers, their polls in flight together
 __device__ __forceinline__ bool wait_three(uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
                                            uint32_t b3, uint32_t p3, int* status, int where) {
   const bool r1 = poll(b1, p1), r2 = poll(b2, p2), r3 = poll(b3, p3);
   if (__all_sync(0xffffffffu, r1 & r2 & r3)) return true;
-  return wait_warp(b1, p1, status, where) && wait_warp(b2, p2, status, where + 10) &&
-         wait_warp(b3, p3, status, where + 11);
+  return wait_inline(b1, p1, status, where) && wait_inline(b2, p2, status, where + 10) &&
+         wait_inline(b3, p3, status, where + 11);
 }
 // The following act for the threads whose `on` is not 0, by predicate: a branch around them
 // costs over a hundred clocks of convergence bookkeeping.
@@ -246,7 +268,6 @@ __device__ __forceinline__ void mma4(uint32_t acc, uint32_t at, uint32_t blo, ui
 struct Cursor {
   const int* off;
   int E, tok, n_tiles;
-  long long pos, end;
   int e, seg, j;
   Split s;
   int row_begin, row_end;
@@ -257,11 +278,9 @@ struct Cursor {
     row_end = hi;
     s = split_rows(hi - lo, tok);
   }
-  __device__ __forceinline__ bool valid() const { return e < E && pos < end; }
   __device__ __forceinline__ int row0() const { return row_begin + seg * s.per; }
   __device__ __forceinline__ int row1() const { return min(row_end, row0() + s.per); }
   __device__ __forceinline__ void next() {
-    ++pos;
     if (++j == n_tiles) {
       j = 0;
       if (++seg == s.n) {
@@ -384,8 +403,6 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   cur.e = __shfl_sync(0xffffffffu, start_sh[0], 0);
   cur.seg = __shfl_sync(0xffffffffu, start_sh[1], 0);
   cur.j = __shfl_sync(0xffffffffu, start_sh[2], 0);
-  cur.pos = __shfl_sync(0xffffffffu, range_sh[0], 0);
-  cur.end = __shfl_sync(0xffffffffu, range_sh[1], 0);
   if (cur.e < a.E) cur.set_expert();
   const int n_out = GATED ? a.N / 2 : a.N;
   // weight row of row r of tile j (clamped into the matrix; what is past it is not stored)
@@ -403,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
   const uint32_t bar_a = smem_u32(bars), bar_freed = bar_a + 8 * kBarFreed, bar_b = bar_a + 8 * kBarB, bar_c = bar_a + 8 * kBarC;
   const uint32_t bar_s = bar_a + 8 * kBarS, bar_acc = bar_a + 8 * kBarAcc, bar_fin = bar_a + 8 * kBarFin;
   const uint32_t one = elect_one();
+  const uint32_t mine = uniform((uint32_t)(range_sh[1] - range_sh[0]));  // tiles of this CTA
   bool ok = true;
 
   if (warp >= 4 && warp < 20) {
@@ -418,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     const uint32_t my_full = bar_a + 8 * (turn * 2 + h), my_freed = bar_freed + 8 * turn;
     const uint32_t my_codes = bar_c + 32 * turn;
     uint32_t n = 0, piece = 0;  // double steps of this turn, pieces of scales so far
-    while (cur.valid() && ok) {
+    for (uint32_t tile = 0; tile < mine && ok; ++tile) {
       for (int k0 = 0; k0 < steps; k0 += kScaleGroups, ++piece) {
         const uint32_t s_bar = bar_s + 16 * (piece & 1);
         uint32_t sat = my_scales + (piece & 1) * kScaleBytes;
@@ -463,14 +481,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
         __syncwarp();
         arrive(s_bar + 8, one);
       }
-      cur.next();
     }
   } else if (warp >= 20) {
     // ------------------------------------------------------------------ results
     const int q = warp & 3;
-    int tile = 0;
     T* out = (T*)a.out;
-    while (cur.valid()) {
+    for (uint32_t tile = 0; tile < mine; ++tile) {
       const int buf = tile & 1;
       ok = wait_warp(bar_acc + 16 * buf, (tile >> 1) & 1, a.status, 61);
       if (!ok) break;
@@ -509,7 +525,6 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
       tc::fence_before_sync();
       __syncwarp();
       arrive(bar_acc + 16 * buf + 8, one);
-      ++tile;
       cur.next();
     }
   } else if (warp == 3) {
@@ -521,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     const uintptr_t bits = (uintptr_t)a.scales | (uintptr_t)a.biases;
     const bool wide = steps % 8 == 0 && bits % 16 == 0, pairs = steps % 2 == 0 && bits % 4 == 0;
     uint32_t buf = 0, ph = 1;
-    while (cur.valid() && ok) {
+    for (uint32_t tile = 0; tile < mine && ok; ++tile) {
       for (int g0 = 0; g0 < steps; g0 += kScaleGroups) {
         ok = wait_warp(bar_s + 16 * buf + 8, ph, a.status, 72);
         if (!ok) break;
@@ -585,14 +600,15 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     const uint32_t base = smem_u32(smem);
     int st = 0, issued = 0;
     uint32_t ph = 1;
-    while (cur.valid() && ok) {
+    for (uint32_t tile = 0; tile < mine && ok; ++tile) {
       // (What lies past the tile's rows is multiplied, and not stored, or not even that. With
       // `tok` rows for every tile the L2 traffic was 1.8 times as much at 106 rows a tile; with
       // several boxes of 32 rows for each tile this warp was too slow, 163 against 147 us.)
-      const int row0 = cur.row0(), boxes = (cur.row1() - row0 + kBoxRows - 1) / kBoxRows;
+      const int row0 = uniform(cur.row0());
+      const int boxes = uniform((cur.row1() - row0 + kBoxRows - 1) / kBoxRows);
       const CUtensorMap* map = &p.x[boxes - 1];
       for (int k = 0; k < steps; k += 2) {
-        ok = wait_warp(bar_b + 16 * st + 8, ph, a.status, 62);
+        ok = wait_inline(bar_b + 16 * st + 8, ph, a.status, 62);
         if (!ok) break;
         const uint32_t dst = base + st * 2 * half_bytes, bar = bar_b + 16 * st;
         const bool both = k + 1 < steps;
@@ -611,14 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     for (int i = min(issued, p.b_stages); i > 0; --i) {
       st = st ? st - 1 : p.b_stages - 1;
       if (st == p.b_stages - 1) ph ^= 1;
-      wait_warp(bar_b + 16 * st, ph ^ 1, a.status, 68);
+      wait_inline(bar_b + 16 * st, ph ^ 1, a.status, 68);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ packed codes
     const uint32_t base = smem_u32(codes);
     uint32_t n[2] = {0, 0};  // double steps of either turn so far
-    while (cur.valid() && ok) {
-      const int row = cur.e * a.N + cur.j * (GATED ? 64 : 128);
+    for (uint32_t tile = 0; tile < mine && ok; ++tile) {
+      const int row = uniform(cur.e * a.N + cur.j * (GATED ? 64 : 128));
       for (int k = 0; k < steps && ok; k += 4) {
 #pragma unroll
         for (int turn = 0; turn < 2; ++turn) {
@@ -626,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
           if (kk < steps && ok) {
             const uint32_t slot = turn * 2 + (n[turn] & 1);
             const uint32_t dst = base + slot * kSlotBytes, bar = bar_c + 16 * slot;
-            ok = wait_warp(bar + 8, (n[turn] >> 1 & 1) ^ 1, a.status, 69);
+            ok = wait_inline(bar + 8, (n[turn] >> 1 & 1) ^ 1, a.status, 69);
             if (ok) {
               arrive_tx(bar, kSlotBytes, one);
               if (GATED) {
@@ -647,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
 #pragma unroll
     for (int turn = 0; turn < 2; ++turn)
       for (uint32_t i = n[turn] < 2 ? 0 : n[turn] - 2; i < n[turn]; ++i)
-        wait_warp(bar_c + 16 * (turn * 2 + (i & 1)), i >> 1 & 1, a.status, 70);
+        wait_inline(bar_c + 16 * (turn * 2 + (i & 1)), i >> 1 & 1, a.status, 70);
   } else if (warp == 0) {
     // ------------------------------------------------------------------ MMA issuer
     // As few instructions as it takes: an MMA or a commit takes its thread 44 clocks.
@@ -656,16 +672,16 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
     const uint32_t dlo = (uint32_t)desc, dhi = (uint32_t)(desc >> 32);
     const uint32_t dhalf = (uint32_t)half_bytes >> 4;  // descriptor units of 16 bytes
     const uint32_t bb_end = bar_b + 16 * p.b_stages;
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    constexpr uint32_t tm = 0;  // all 512 columns are taken, so they begin at 0
     uint32_t bb = bar_b, blo = dlo;  // full barrier and descriptor of the B stage
-    uint32_t bph = 0, aph = 0, tile = 0;  // bit t of aph: phase of turn t
+    uint32_t bph = 0, aph = 0;  // bit t of aph: phase of turn t
     uint32_t ready = 0;  // the next double step's barriers, tested while this one's MMAs run
-    while (cur.valid() && ok) {
-      const int rows = cur.row1() - cur.row0();
+    for (uint32_t tile = 0; tile < mine && ok; ++tile) {
+      const int rows = uniform(cur.row1() - cur.row0());
       const uint32_t idesc = tc::idesc_f16(kBf, 128, 0, false, false) +
                              ((uint32_t)((rows + 15) / 16 * 2) << 17);
       const uint32_t buf = tile & 1, acc = tm + buf * kMaxTok;
-      ok = wait_warp(bar_acc + 16 * buf + 8, (tile >> 1 & 1) ^ 1, a.status, 63);
+      ok = wait_inline(bar_acc + 16 * buf + 8, (tile >> 1 & 1) ^ 1, a.status, 63);
       uint32_t turn = 0;
       for (int k = 0; k < steps && ok; k += 2) {
         const uint32_t ba = bar_a + 16 * turn, ph = aph >> turn & 1;
@@ -693,13 +709,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
         commit(b_free, one);
         if (last) commit(bar_acc + 16 * buf, one);
       }
-      ++tile;
       cur.next();
     }
     // every MMA has completed before tensor memory is freed (one lane, the same each time,
     // issued them all)
     commit(bar_fin, one);
-    wait_warp(bar_fin, 0, a.status, 66);
+    wait_inline(bar_fin, 0, a.status, 66);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -711,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_tc_kernel(const __grid_con
 // product kernel could gather by itself, but four-row TMA loads and 16-byte cp.async both
 // brought 32 bytes a clock and SM where its MMAs take 64 (16384 rows of 2048 through 128 experts
 // of 1536x2048: 185 us with gathering inside; 13 us for this kernel, which writes 67 MB,
-// and 130 for the product).
+// and 128 for the product).
 __global__ void __launch_bounds__(256)
     gather_rows_kernel(const uint4* __restrict__ x, long long ldx, int x_rows,
                        const int* __restrict__ rows, uint4* __restrict__ out, int R, int per_row) {
