@@ -10,8 +10,10 @@
 // earlier tokens that took it: a popcount over a per-expert bit mask of tokens. Counts and
 // masks are integers, so the order of their atomics does not show.
 //
-// What bounds it: a decode batch is one block's latency; a long chunk reads the logits once
-// (HBM) and then the counts of the earlier blocks (L2).
+// What bounds it: a decode batch is one block's latency (16 tokens of 128 experts 4.5 us); a
+// long chunk reads the logits once (HBM) and then the counts of the earlier blocks (L2), and is
+// bound by the chains of warp reductions of a token's choice (8192 tokens of 256 experts in fp32
+// 18.5 us, two thirds of it the choices; the 8.4 MB of logits take 1.3).
 #include <algorithm>
 
 #include "matmul_internal.h"
@@ -314,6 +316,9 @@ constexpr int kOneBlock = 64;
 
 size_t place_smem(int E, int bt) { return (size_t)(2 * E + 1 + (bt + 31) / 32 * E) * sizeof(int); }
 
+// Bound by HBM: 2048 tokens of 8 rows of 2048 with a residual 19.5 us, 4.3 of 6.6 TB/s; the rows
+// come in the order of the experts, 4 KB at a time.
+//
 // out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]], in fp32, j in order; a slot
 // outside [0, R) adds nothing. VEC values per thread.
 template <typename T, int VEC>

@@ -484,6 +484,8 @@ def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int
         _check_out(out, (*shape[:-1], n_out), x)
     elif len(shape) == 2:
         out = _empty((m, n_out), (n_out, 1), tp)
+    elif len(shape) == 3:
+        out = _empty((shape[0], shape[1], n_out), (shape[1] * n_out, n_out, 1), tp)
     else:
         out = x.new_empty((*shape[:-1], n_out))
     check(_lib.fn("qkv_quantized_matmul")(
