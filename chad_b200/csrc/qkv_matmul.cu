@@ -106,10 +106,13 @@ __device__ __forceinline__ void cp_small(uint32_t dst, const void* src) {
 
 // The expert and the first row of token chunk `id` (chunks of `per` rows, experts in order),
 // by a whole warp; false past the last chunk. Offsets are clamped into [0, R], and a
-// decreasing pair counts as an empty expert, so bad offsets cannot leave the tensors.
+// decreasing pair counts as an empty expert, so bad offsets cannot leave the tensors. (With pairs
+// that decrease the other experts can have any part of the R rows each, so chunks are counted in
+// 64 bits.)
 __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int E, int R, int per,
-                                           int id, int lane, int& expert, int& row0, int& row1) {
-  int base = 0;
+                                           long long id, int lane, int& expert, int& row0,
+                                           int& row1) {
+  long long base = 0;
   for (int e0 = 0; e0 < E; e0 += 32) {
     const int e = e0 + lane;
     int lo = 0, hi = 0;
@@ -118,10 +121,10 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
       hi = min(max(offsets[e + 1], 0), R);
     }
     const int n = hi > lo ? (hi - lo + per - 1) / per : 0;
-    int sum = n;
+    long long sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      const long long v = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += v;
     }
     const bool here = id < base + sum && id >= base + sum - n;
@@ -129,7 +132,7 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
     if (m) {
       const int src = __ffs(m) - 1;
       expert = e0 + src;
-      const int first = __shfl_sync(0xffffffffu, lo + (id - (base + sum - n)) * per, src);
+      const int first = __shfl_sync(0xffffffffu, lo + (int)(id - (base + sum - n)) * per, src);
       const int end = __shfl_sync(0xffffffffu, hi, src);
       row0 = first;
       row1 = min(first + per, end);
@@ -141,14 +144,16 @@ __device__ __forceinline__ bool find_chunk(const int* __restrict__ offsets, int 
 }
 
 // How many token chunks there are, by a whole warp.
-__device__ __forceinline__ int count_chunks(const int* __restrict__ offsets, int E, int R, int per,
-                                            int lane) {
-  int n = 0;
+__device__ __forceinline__ long long count_chunks(const int* __restrict__ offsets, int E, int R,
+                                                  int per, int lane) {
+  long long n = 0;
   for (int e = lane; e < E; e += 32) {
     const int lo = min(max(offsets[e], 0), R), hi = min(max(offsets[e + 1], 0), R);
     n += hi > lo ? (hi - lo + per - 1) / per : 0;
   }
-  return __reduce_add_sync(0xffffffffu, n);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
 }
 
 constexpr int kStages = 3;                  // of one chunk, per warp
@@ -165,7 +170,6 @@ struct RowsArgs {
   int wk_count;  // warps that share K
   int tiles;     // of 16 weight rows
   int per;       // rows of x per CTA (at most 8)
-  int most;      // chunks of `per` rows that the experts can have
 };
 
 // GATED: MMA rows 0-7 are gate rows, 8-15 the up rows of the same outputs. SB: how a row's four
@@ -175,6 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][kWarps][4][32];
   __shared__ int seg[3], sums_of[kWarps];
+  __shared__ long long count_of;
   // everything here may come from the kernel before, the weights too
   wait_for_previous();
   const MatmulArgs& a = p.a;
@@ -192,19 +197,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const uint32_t ring = zeros + 128 + warp * kStages * kStageBytes;
   // This CTA's units: every gridDim.x-th of its chunk of rows, or with experts an equal run of
   // those of all their chunks, whose number only the device knows.
-  int lo, hi, id = blockIdx.y;
+  int unit0 = blockIdx.x, left = 0;  // the first unit, and with experts how many
+  long long id = blockIdx.y;
   int my_lo = 0, my_hi = 0, my_n = 0, my_id = 0;  // rows, chunks and first chunk of expert threadIdx.x
   const bool few = a.E <= kWarps * 32;            // a thread for every expert
   if (GROUPED) {
     if (threadIdx.x < 3) seg[threadIdx.x] = 0;
-    int all = 0;
+    long long all = 0;
     if (few) {
       if ((int)threadIdx.x < a.E) {
         my_lo = min(max(a.offsets[threadIdx.x], 0), a.R);
         my_hi = min(max(a.offsets[threadIdx.x + 1], 0), a.R);
         my_n = my_hi > my_lo ? (my_hi - my_lo + p.per - 1) / p.per : 0;
       }
-      int sum = my_n;
+      int sum = my_n;  // (256 experts' chunks in 32 bits: more rows go to the other kernel)
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -220,36 +226,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       }
     } else {
       if (warp == 0) {
-        const int n = count_chunks(a.offsets, a.E, a.R, p.per, lane);
-        if (lane == 0) sums_of[0] = n;
+        const long long n = count_chunks(a.offsets, a.E, a.R, p.per, lane);
+        if (lane == 0) count_of = n;
       }
       __syncthreads();
-      all = sums_of[0];
+      all = count_of;
     }
-    // (offsets that decrease may count more chunks than there can be)
-    all = min(__shfl_sync(0xffffffffu, all, 0), p.most) * units;
-    const int each = all / (int)gridDim.x, left = all - each * (int)gridDim.x, b = blockIdx.x;
-    lo = b * each + min(b, left);
-    hi = lo + each + (b < left ? 1 : 0);
-    if (lo >= hi) return;
+    all = __shfl_sync(0xffffffffu, all, 0) * units;
+    const long long lo = all * blockIdx.x / gridDim.x;
+    left = (int)(all * (blockIdx.x + 1) / gridDim.x - lo);
+    if (left == 0) return;
     id = lo / units;
-  } else {
-    lo = 0;
-    hi = units;
+    unit0 = (int)(lo - id * units);
   }
 
   int buf = 0;
-  for (int first = GROUPED ? id * units : 0; first < hi; first += units, ++id) {
-    const int unit0 = GROUPED ? max(lo - first, 0) : blockIdx.x;
-    const int unit1 = GROUPED ? min(hi - first, units) : units;
+  do {
+    const int unit1 = GROUPED ? min(unit0 + left, units) : units;
     const int step = GROUPED ? 1 : gridDim.x;
     int expert = 0, row0, row1;
     if (GROUPED) {
       if (few) {
         if (id >= my_id && id < my_id + my_n) {
           seg[0] = threadIdx.x;
-          seg[1] = my_lo + (id - my_id) * p.per;
-          seg[2] = min(my_lo + (id - my_id + 1) * p.per, my_hi);
+          seg[1] = my_lo + (int)(id - my_id) * p.per;
+          seg[2] = min(my_lo + (int)(id - my_id + 1) * p.per, my_hi);
         }
       } else if (warp == 0) {
         int e = 0, r0 = 0, r1 = 0;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       row0 = __shfl_sync(0xffffffffu, seg[1], 0);
       row1 = __shfl_sync(0xffffffffu, seg[2], 0);
     } else {
-      row0 = id * p.per;
+      row0 = (int)id * p.per;
       row1 = min(row0 + p.per, a.R);
     }
     const int rows = row1 - row0;
@@ -466,7 +467,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       }
       if (wk == 0 && tile < p.tiles) store(tile, acc);
     }
-  }
+    if (!GROUPED) break;
+    left -= unit1 - unit0;
+    unit0 = 0;
+    ++id;
+  } while (left > 0);
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
@@ -534,7 +539,6 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   p.wk_count = best;
   const int units = (p.tiles + kWarps / best - 1) / (kWarps / best);
   if (a.offsets && segs * units > 1ll << 30) return QKV_EUNSUPPORTED;
-  p.most = (int)std::min<long long>(segs, 0x7fffffff);
   const dim3 grid =
       a.offsets ? dim3((unsigned)std::min<long long>(resident, segs * units))
                 : dim3((unsigned)std::min<long long>(units, std::max(1ll, resident / segs)),

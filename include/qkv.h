@@ -275,8 +275,8 @@ int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void
  *
  * w (E, N, K/8), scales and biases (E, N, K/64), offsets device int32[E+1] (ascending, within
  * [0, R]), rows device int32[R] or NULL. Rows of out outside [offsets[0], offsets[E]) are not
- * written. Offsets outside [0, R] are clamped and a decreasing pair is an empty expert (rows
- * that it leaves to two experts hold either's result); an entry of rows outside [0, x_rows)
+ * written. Offsets outside [0, R] are clamped and a decreasing pair is an empty expert (of rows
+ * that it leaves to two experts each value is either's); an entry of rows outside [0, x_rows)
  * reads a row of zeros.
  */
 int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows,
