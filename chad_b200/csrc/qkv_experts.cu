@@ -15,6 +15,7 @@
 // bound by the chains of warp reductions of a token's choice (8192 tokens of 256 experts in fp32
 // 18.5 us, two thirds of it the choices; the 8.4 MB of logits take 1.3).
 #include <algorithm>
+#include <atomic>
 
 #include "matmul_internal.h"
 #include "qkv_common.cuh"
@@ -409,13 +410,19 @@ static int launch_route_t(const RouteArgs& a, cudaStream_t st) {
   const int bt = route_block_tokens(a.T), place = bt * kPlaceBlocks;
   const unsigned blocks = (unsigned)((a.T + bt - 1) / bt);
   const size_t smem = place_smem(a.E, place);
-  // (the bound is the same for every call: another thread's may come before this launch)
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(route_place_kernel<false, QKV_F32>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)place_smem(kMaxRouteExperts, kMaxBlockTokens * kPlaceBlocks)) !=
-          cudaSuccess)
-    return QKV_ECUDA;
+  // Set on a device's first call, whatever its sizes: the bound that holds without it counts the
+  // kernel's static bytes as well.
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ECUDA;
+  if (dev < 0 || dev >= kMaxDevices || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(route_place_kernel<false, QKV_F32>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)place_smem(kMaxRouteExperts, kMaxBlockTokens * kPlaceBlocks)) !=
+        cudaSuccess)
+      return QKV_ECUDA;
+    if (dev >= 0 && dev < kMaxDevices) ready.fetch_or(1ull << dev);
+  }
   const int rc = launch(true, route_choose_kernel<DTYPE>, dim3(blocks), kChooseThreads,
                                   a.E * sizeof(int), st, a, bt);
   if (rc) return rc;
