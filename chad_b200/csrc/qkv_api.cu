@@ -43,6 +43,15 @@ int cuda_check(const char* what) {
   return QKV_OK;
 }
 
+// The result of a launcher: the CUDA error behind QKV_ECUDA is named, and read, so that the
+// thread's next call does not report it; without one a tensor map was refused by the driver.
+int launched(int rc, const char* what, const char* unsupported) {
+  if (rc == QKV_OK) return cuda_check(what);
+  if (rc != QKV_ECUDA) return fail(rc, "%s", unsupported);
+  const cudaError_t e = cudaGetLastError();
+  return fail(rc, "%s: %s", what, e != cudaSuccess ? cudaGetErrorString(e) : "tensor map refused");
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int* status_ptr() {
@@ -165,8 +174,7 @@ int qkv_quantize_append(const void* x, int x_dtype, void* w, void* scales, void*
   if (rc) return rc;
   rc = launch_quantize(x, x_dtype, w, scales, biases, B, H, S, D, NP, offset, bits, scale_dtype,
                        static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "quantize: unsupported shape");
-  return cuda_check("qkv_quantize_append");
+  return launched(rc, "qkv_quantize_append", "quantize: unsupported shape");
 }
 
 int qkv_quantize_append_kv(const void* k, const void* v, int x_dtype, void* kw, void* ks,
@@ -185,8 +193,7 @@ int qkv_quantize_append_kv(const void* k, const void* v, int x_dtype, void* kw, 
   void* bs[2] = {kb, vb};
   rc = launch_quantize_jobs(xs, x_dtype, ws_, ss, bs, 2, B, H, S, D, NP, offset, bits,
                             scale_dtype, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "quantize: unsupported shape");
-  return cuda_check("qkv_quantize_append_kv");
+  return launched(rc, "qkv_quantize_append_kv", "quantize: unsupported shape");
 }
 
 int qkv_dequantize(const void* w, const void* scales, const void* biases, void* out,
@@ -200,8 +207,7 @@ int qkv_dequantize(const void* w, const void* scales, const void* biases, void* 
   if (round_mode != 0 && round_mode != 1) return fail(QKV_EINVAL, "bad round_mode %d", round_mode);
   rc = launch_dequantize(w, scales, biases, out, rows, D, bits, dtype, round_mode,
                          static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "dequantize: unsupported shape");
-  return cuda_check("qkv_dequantize");
+  return launched(rc, "qkv_dequantize", "dequantize: unsupported shape");
 }
 
 size_t qkv_workspace_size(int B, int HQ, int HKV, int S, int D, int n_max, int bits,
@@ -352,8 +358,7 @@ int qkv_attention(const void* q, const void* kw, const void* ks, const void* kb,
   a.out_kind = out_kind;
   rc = a.use_tc ? launch_prefill_tc(a, a.tc, true, static_cast<cudaStream_t>(stream))
                 : launch_decode(a, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "attention: unsupported configuration");
-  return cuda_check("qkv_attention");
+  return launched(rc, "qkv_attention", "attention: unsupported configuration");
 }
 
 int qkv_partials(const void* q, const void* kw, const void* ks, const void* kb, const void* vw,
@@ -374,8 +379,7 @@ int qkv_partials(const void* q, const void* kw, const void* ks, const void* kb, 
   *n_parts = a.use_tc ? a.tc.parts : a.splits;
   rc = a.use_tc ? launch_prefill_tc(a, a.tc, false, static_cast<cudaStream_t>(stream))
                 : launch_split_only(a, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "partials: unsupported configuration");
-  return cuda_check("qkv_partials");
+  return launched(rc, "qkv_partials", "partials: unsupported configuration");
 }
 
 int qkv_combine(const float* parts, int n_parts, long long rows, int D, void* out, int out_dtype,
@@ -389,8 +393,7 @@ int qkv_combine(const float* parts, int n_parts, long long rows, int D, void* ou
   const int rc =
       launch_combine(parts, n_parts, rows, rows, D, out, out_dtype, out_kind,
                      static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "combine: unsupported");
-  return cuda_check("qkv_combine");
+  return launched(rc, "qkv_combine", "combine: unsupported");
 }
 
 int qkv_prefill(const void* q, const void* k_new, const void* v_new, void* kw, void* ks, void* kb,
@@ -426,11 +429,10 @@ int qkv_prefill(const void* q, const void* k_new, const void* v_new, void* kw, v
     void* bs[2] = {kb, vb};
     rc = launch_quantize_jobs(xs, dtype, ws_, ss, bs, 2, B, HKV, S, D, NP, offset, bits, dtype,
                               st);
-    if (rc) return fail(rc, "quantize: unsupported shape");
+    if (rc) return launched(rc, "qkv_prefill", "quantize: unsupported shape");
     rc = a.use_tc ? launch_prefill_tc(a, a.tc, true, st) : launch_decode(a, st);
   }
-  if (rc) return fail(rc, "prefill: unsupported configuration");
-  return cuda_check("qkv_prefill");
+  return launched(rc, "qkv_prefill", "prefill: unsupported configuration");
 }
 
 namespace {
@@ -512,8 +514,7 @@ int qkv_quantized_matmul(const void* x, long long ldx, const void* w, const void
                         group_size, dtype, act, workspace, ws_bytes);
   if (rc || M == 0) return rc;
   rc = launch_matmul(a, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "quantized_matmul: unsupported shape");
-  return cuda_check("qkv_quantized_matmul");
+  return launched(rc, "qkv_quantized_matmul", "quantized_matmul: unsupported shape");
 }
 
 int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows,
@@ -529,8 +530,7 @@ int qkv_grouped_matmul(const void* x, long long ldx, int x_rows, const int* rows
                         bits, group_size, dtype, act, workspace, ws_bytes);
   if (rc || R == 0) return rc;
   rc = launch_matmul(a, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "grouped_matmul: unsupported shape");
-  return cuda_check("qkv_grouped_matmul");
+  return launched(rc, "qkv_grouped_matmul", "grouped_matmul: unsupported shape");
 }
 
 size_t qkv_route_workspace_size(int T, int E) {
@@ -559,8 +559,7 @@ int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int norma
   const RouteArgs a = {logits, dtype, T, E, k, normalize, experts, weights, rows, slots, offsets,
                        (int*)workspace};
   const int rc = launch_route(a, static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "route: launch failed");
-  return cuda_check("qkv_route_topk");
+  return launched(rc, "qkv_route_topk", "route: launch failed");
 }
 
 int qkv_expert_combine(const void* y, int R, const int* slots, const float* weights,
@@ -580,8 +579,7 @@ int qkv_expert_combine(const void* y, int R, const int* slots, const float* weig
     return fail(QKV_EINVAL, "out overlaps the residual without being it");
   const int rc = launch_expert_combine(y, R, slots, weights, residual, out, T, k, N, dtype,
                                        static_cast<cudaStream_t>(stream));
-  if (rc) return fail(rc, "expert_combine: unsupported shape");
-  return cuda_check("qkv_expert_combine");
+  return launched(rc, "qkv_expert_combine", "expert_combine: unsupported shape");
 }
 
 }  // extern "C"

@@ -26,3 +26,37 @@ def test_route_just_below_48_kib_of_masks_first(t, e, k):
           "t, e, k = map(int, sys.argv[1:])\n"
           "gen = torch.Generator().manual_seed(t)\n"
           "check_route(torch.randn(t, e, generator=gen).to(torch.bfloat16).cuda(), k, True)\n", t, e, k)
+
+
+def test_a_refused_launch_is_not_reported_by_the_next_call():
+    """A call into an invalidated capture is refused with the CUDA error; the next one succeeds."""
+    fresh("""
+import torch
+from chad_b200 import ops
+from chad_b200._lib import QKVError
+y = torch.ones(8, 64, dtype=torch.bfloat16, device="cuda")
+slots = torch.arange(8, dtype=torch.int32, device="cuda").view(4, 2)
+weights, out = torch.ones(4, 2, device="cuda"), torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+ops.expert_combine(y, slots, weights, out=out)
+torch.cuda.synchronize()
+stream, graph, said = torch.cuda.Stream(), torch.cuda.CUDAGraph(), ""
+with torch.cuda.stream(stream):
+    graph.capture_begin(capture_error_mode="thread_local")
+    try:
+        stream.synchronize()  # not allowed while capturing: the capture is invalid from here on
+    except RuntimeError:
+        pass
+    try:
+        ops.expert_combine(y, slots, weights, out=out)
+    except QKVError as error:
+        said = str(error)
+    try:
+        graph.capture_end()
+    except RuntimeError:
+        pass
+assert "capture" in said and "unsupported shape" not in said, said
+out.zero_()
+ops.expert_combine(y, slots, weights, out=out)
+torch.cuda.synchronize()
+assert bool((out == 2).all())
+""")

@@ -132,3 +132,13 @@ def test_python_bindings_return_the_librarys_codes():
     assert ext.expert_combine(16, 32, 16, 16, None, 16, 4, 8, 64, 2, None) == EINVAL
     with pytest.raises(TypeError):
         ext.route_topk(16)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch on addresses that are none")
+@pytest.mark.parametrize("call", [_matmul, _grouped, _route, _combine])
+def test_a_refused_launch_names_the_cuda_error(call):
+    lib = _lib.load()
+    assert call(lib) == _lib.QKV_ECUDA
+    message = lib.qkv_last_error().decode()
+    assert "unsupported" not in message and "launch failed" not in message
+    assert message.startswith("qkv_"), message
