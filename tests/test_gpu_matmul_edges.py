@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from chad_b200 import ops
-from tests.test_gpu_matmul import check, make_weights, reference
+from tests.test_gpu_matmul import check, make_weights, reference, takes_many
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,27 @@ def test_rows_of_experts_that_overlap(offsets, empty):
             right[a:b] |= ((out[a:b].double() - want).abs() <= err)
             held[a:b] = True
     assert torch.equal(right, held[:, None].expand_as(right)) and bool(out[~held].isnan().all())
+
+
+@pytest.mark.parametrize("m", [1, 4000])
+def test_gates_far_below_zero(m):
+    """silu of -80 to -88 times a large up projection: about 2^-126 times 2^70, not zero.
+
+    One-hot rows and weights of whole steps, so that gate and up are exact; the largest argument of
+    expf is 88, inside its range, and 2^-21 covers it, the divide and two products as in `reference`.
+    """
+    n, k, dt = 1024, 128, torch.bfloat16
+    assert takes_many(m, 1, n, k) == (m > 1)
+    half = n // 2
+    w = torch.zeros(n, k // 8, dtype=torch.int32, device="cuda")  # every weight is its bias
+    s = torch.ones(n, k // 64, dtype=dt, device="cuda")
+    b = torch.empty(n, k // 64, dtype=dt, device="cuda")
+    b[:half] = -80 - 0.5 * (torch.arange(half, device="cuda") % 17).to(dt)[:, None]
+    b[half:] = 2.0 ** 70
+    x = torch.zeros(m, k, dtype=dt, device="cuda")
+    x[torch.arange(m), torch.arange(m) % k] = 1
+    got = ops.quantized_matmul(x, (w, s, b), activation="swiglu").double()
+    gate = b[:half, 0].double()
+    want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 70).expand(m, half)
+    assert bool((gate == -88).any())
+    assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs()).all())
