@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
   const uint32_t ring = zeros + 128 + warp * kStages * kStageBytes;
   // This CTA's units: every gridDim.x-th of its chunk of rows, or with experts an equal run of
   // those of all their chunks, whose number only the device knows.
-  int unit0 = blockIdx.x, left = 0;  // the first unit, and with experts how many
-  long long id = blockIdx.y;
+  int lo = 0, hi = units, id = blockIdx.y;  // units counted from chunk `id`, `from` with experts
+  long long from = 0;
   int my_lo = 0, my_hi = 0, my_n = 0, my_id = 0;  // rows, chunks and first chunk of expert threadIdx.x
   const bool few = a.E <= kWarps * 32;            // a thread for every expert
   if (GROUPED) {
@@ -233,28 +233,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       all = count_of;
     }
     all = __shfl_sync(0xffffffffu, all, 0) * units;
-    const long long lo = all * blockIdx.x / gridDim.x;
-    left = (int)(all * (blockIdx.x + 1) / gridDim.x - lo);
-    if (left == 0) return;
-    id = lo / units;
-    unit0 = (int)(lo - id * units);
+    const long long each = all / gridDim.x, first = blockIdx.x * each;
+    const int more = (int)(all - each * gridDim.x), b = blockIdx.x;  // CTAs with one unit more
+    from = (first + min(b, more)) / units;
+    id = 0;
+    lo = (int)(first + min(b, more) - from * units);
+    hi = lo + (int)each + (b < more ? 1 : 0);
+    if (lo >= hi) return;
+    my_id -= (int)from;
   }
 
   int buf = 0;
-  do {
-    const int unit1 = GROUPED ? min(unit0 + left, units) : units;
+  for (int first = 0; first < hi; first += units, ++id) {
+    const int unit0 = GROUPED ? max(lo - first, 0) : blockIdx.x;
+    const int unit1 = GROUPED ? min(hi - first, units) : units;
     const int step = GROUPED ? 1 : gridDim.x;
     int expert = 0, row0, row1;
     if (GROUPED) {
       if (few) {
         if (id >= my_id && id < my_id + my_n) {
           seg[0] = threadIdx.x;
-          seg[1] = my_lo + (int)(id - my_id) * p.per;
-          seg[2] = min(my_lo + (int)(id - my_id + 1) * p.per, my_hi);
+          seg[1] = my_lo + (id - my_id) * p.per;
+          seg[2] = min(my_lo + (id - my_id + 1) * p.per, my_hi);
         }
       } else if (warp == 0) {
         int e = 0, r0 = 0, r1 = 0;
-        find_chunk(a.offsets, a.E, a.R, p.per, id, lane, e, r0, r1);
+        find_chunk(a.offsets, a.E, a.R, p.per, from + id, lane, e, r0, r1);
         if (lane == 0) {
           seg[0] = e;
           seg[1] = r0;
@@ -266,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       row0 = __shfl_sync(0xffffffffu, seg[1], 0);
       row1 = __shfl_sync(0xffffffffu, seg[2], 0);
     } else {
-      row0 = (int)id * p.per;
+      row0 = id * p.per;
       row1 = min(row0 + p.per, a.R);
     }
     const int rows = row1 - row0;
@@ -467,11 +471,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) matmul_rows_kernel(const RowsA
       }
       if (wk == 0 && tile < p.tiles) store(tile, acc);
     }
-    if (!GROUPED) break;
-    left -= unit1 - unit0;
-    unit0 = 0;
-    ++id;
-  } while (left > 0);
+  }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
