@@ -165,6 +165,15 @@ constexpr int kStageBytes = kCodeBytes + 2 * 16 * 8;  // and four scales and bia
 constexpr int kDynamicBytes = 227 * 1024 - 8192 - 256;
 inline long long x_bytes(int rows, int K) { return (long long)rows * K * 2 + (long long)K / 64 * 32 + 128; }
 
+// Rows of x in one pass over the weights: eight, or as many as fit beside the rings (0: not one).
+// (Two or four tiles of eight rows to a pass were slower at every row count: 2048x4096 at 64 rows
+// 15.4 us with one tile, 15.5 and 21.8 with two and four; 12288x2048 at 32 rows 18.8, 17.8, 28.5.)
+int rows_per_pass(int R, int K) {
+  int per = std::min(8, R);
+  while (per > 0 && x_bytes(per, K) + kWarps * kStages * kStageBytes > kDynamicBytes) --per;
+  return per;
+}
+
 struct RowsArgs {
   MatmulArgs a;
   int wk_count;  // warps that share K
@@ -506,11 +515,7 @@ int launch_rows(const MatmulArgs& a, cudaStream_t st) {
   RowsArgs p;
   p.a = a;
   p.tiles = gated ? (n_out + 7) / 8 : (n_out + 15) / 16;
-  // Eight rows, or as many as fit beside the rings. (Two or four tiles of eight rows to a pass
-  // over the weights were slower at every row count: 2048x4096 at 64 rows 15.4 us with one tile,
-  // 15.5 and 21.8 with two and four; 12288x2048 at 32 rows 18.8, 17.8 and 28.5.)
-  p.per = std::min(8, a.R);
-  while (p.per > 0 && x_bytes(p.per, a.K) + kWarps * kStages * kStageBytes > kDynamicBytes) --p.per;
+  p.per = rows_per_pass(a.R, a.K);
   if (p.per < 1) return QKV_EUNSUPPORTED;
   long long segs = (a.R + p.per - 1ll) / p.per;
   if (a.offsets) segs = std::min<long long>(a.R, std::min(a.E, a.R) + segs);
@@ -557,21 +562,32 @@ int launch_matmul_rows(const MatmulArgs& a, cudaStream_t st) {
   return launch_rows<__half>(a, st);
 }
 
-// Few rows go to the kernel above, which reads the weights once per eight rows; the tcgen05
-// kernel reads them once, but takes 6 us and 2.6 for every 1024 of K and round of 128 x 192 tiles
-// over the SMs, the other 4 and 1 for every 8 million weights of a pass (both measured, to 15%).
-// us of this and of that kernel at 16, 32, 64 and 96 rows: 2048x4096 6.8 9.2 13.7 18.6, 16.7 17.0
-// 17.7 18.8; 5120x2048 8.3 10.9 16.0 19.9, 11.4 11.6 12.1 12.8; 12288x2048 11.4 16.9 27.3 34.9,
-// 11.9 12.1 12.8 13.5; 2048x16384 25.7 42.4 79.1 105, 49.4 50.2 51.8 54.7. Experts' rows are
-// no more than 8 each up to R = 8 E, whatever the sizes then: 4, 8 and 12 rows for each of 64
-// experts of 1536x2048 30.9 41.8 53.2, 39.1 44.9 45.7; 8 and 10 for each of 128 73.1 85.0, 75.0 77.8.
+// Few rows go to the kernel above, which takes a pass over the weights for every rows_per_pass
+// rows; the tcgen05 kernel reads them once, but takes 6 us and 2.6 for every 1024 of K and round of
+// 128 x 192 tiles over the SMs, the other 4 and 1 for every 8 million weights of a pass (both
+// measured, to 15%).
+// us of this and of that kernel at 16, 32, 64 and 96 rows: 2048x4096 6.9 9.1 13.4 18.3, 16.8 17.0
+// 17.3 17.8; 5120x2048 8.4 10.9 15.5 19.7, 11.3 11.4 11.8 12.3; 12288x2048 11.5 16.8 27.3 34.6,
+// 12.2 12.4 12.8 13.4. At 4, 8, 12 and 16 rows of long K: 8192x14336 (five rows a pass) 22.3 35.2
+// 50.4 59.5, 46.3 throughout; 8192x28672 (two) 64.9 114 172 232, 88.0; 5120x28672 49.3 79.8 113
+// 143, 86.8; 2048x28672 24.6 39.3 53.8 67.5, 86.2.
+// Experts' counts are on the device. With the counts of routed tokens both kernels take the same
+// time at about ten rows on average, or earlier where some experts are popular (us of this and of
+// that kernel at 8, 10 and 12 rows for each of the experts on average; logits normal, "popular" with
+// as much again by expert): 128 of 1536x2048 gated 69.7 82.4 92.9, 83.9 84.3 84.5, popular 68.2 75.7
+// 88.5, 62.9 67.4 67.9; 64 of these 40.7 42.7 54.0, 52.0 52.2 52.4, popular 40.2 42.8 52.4, 40.4
+// 41.0 46.3; 32 of these 22.5 25.7 30.5, 32.7 32.7 32.8; 128 of 2048x768 39.0 45.3 49.7, 49.2 49.5
+// 49.4, popular 38.3 42.4 48.0, 37.2 41.6 40.7; 60 of 2048x1408 39.0 41.6 48.2, 44.1 44.3 44.7.
 bool matmul_takes_tc(int R, int E, int N, int K) {
   if (!matmul_tc_fits(E, N)) return false;
-  if (K > 65536) return true;  // a row of x does not fit shared memory beside the rings above
+  const int per = rows_per_pass(R, K);
+  if (per < 1) return true;  // a row of x does not fit shared memory beside the rings above
   if (R > 65528) return true;  // the kernel above has one grid row for every eight at most
-  if (R <= 8ll * std::min(E, R)) return false;
-  const long long passes = (R + 7ll) / 8, tiles = (N + 127ll) / 128 * ((R + 191ll) / 192);
-  return passes * N > 16000000 / K + 20000 * ((tiles + 147) / 148);
+  const int experts = std::min(E, R);
+  if (R <= (long long)per * experts || (experts > 1 && 4ll * R <= 5ll * per * experts)) return false;
+  const long long passes = (R + per - 1ll) / per, sms = num_sms();
+  const long long tiles = (N + 127ll) / 128 * ((R + 191ll) / 192);
+  return passes * N > 16000000 / K + 20000 * ((tiles + sms - 1) / sms);
 }
 
 int launch_matmul(const MatmulArgs& a, cudaStream_t st) {

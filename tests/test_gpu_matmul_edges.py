@@ -57,3 +57,26 @@ def test_gates_far_below_zero(m):
     want = (gate / (1 + torch.exp(-gate)) * 2.0 ** 70).expand(m, half)
     assert bool((gate == -88).any())
     assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs()).all())
+
+
+@pytest.mark.parametrize("m,k", [(1, 67392), (2, 67392), (1, 67456), (9, 14336), (5, 28672)])
+def test_longest_rows_beside_the_weights_stages(m, k):
+    gen = torch.Generator().manual_seed(k + m)
+    wq = make_weights(gen, (40,), k, torch.bfloat16)
+    x = torch.randn(m, k, generator=gen).bfloat16().cuda()
+    want, err = reference(x, wq, None, torch.bfloat16)
+    check(ops.quantized_matmul(x, wq), want, err, f"{m} rows of {k}")
+
+
+@pytest.mark.parametrize("k", [14336, 28672, 67392])
+def test_experts_with_fewer_rows_to_a_pass(k):
+    gen = torch.Generator().manual_seed(k)
+    counts = [3, 0, 7, 1, 2]
+    wq = make_weights(gen, (5, 24), k, torch.bfloat16)
+    offsets = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    x = torch.randn(sum(counts), k, generator=gen).bfloat16().cuda()
+    got = ops.grouped_quantized_matmul(x, wq, offsets)
+    for i, (a, b) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:])):
+        if a < b:
+            want, err = reference(x[a:b], [t[i] for t in wq], None, torch.bfloat16)
+            check(got[a:b], want, err, f"expert {i}")
