@@ -75,6 +75,9 @@ class QuantizedExperts:
     def __call__(self, x: torch.Tensor, logits: torch.Tensor,
                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x (T, K), router logits (T, E) -> (residual +) the experts' weighted sum (T, K)."""
+        if x.dim() != 2 or logits.dim() != 2 or logits.shape[0] != x.shape[0]:
+            raise ValueError(f"x {tuple(x.shape)} and logits {tuple(logits.shape)} must be (T, K) "
+                             "and (T, E) of the same tokens")
         r = ops.route_topk(logits, self.top_k, normalize=self.normalize)
         h = ops.grouped_quantized_matmul(x, self.gate_up, r.offsets, rows=r.rows,
                                          activation="swiglu")

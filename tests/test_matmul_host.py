@@ -142,3 +142,13 @@ def test_a_refused_launch_names_the_cuda_error(call):
     message = lib.qkv_last_error().decode()
     assert "unsupported" not in message and "launch failed" not in message
     assert message.startswith("qkv_"), message
+
+
+@pytest.mark.parametrize("x,logits", [((3, 128), (2, 4)), ((2, 128), (3, 4)), ((1, 2, 128), (2, 4)),
+                                      ((2, 128), (4,))])
+def test_experts_layer_refuses_logits_of_other_tokens(x, logits):
+    e = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    layer = experts.QuantizedExperts((e(4, 128, 16, dt=torch.int32), e(4, 128, 2), e(4, 128, 2)),
+                                     (e(4, 128, 8, dt=torch.int32), e(4, 128, 1), e(4, 128, 1)), 2)
+    with pytest.raises(ValueError, match="same tokens"):
+        layer(e(*x), e(*logits))
