@@ -1,6 +1,7 @@
 // C-ABI entry points of libqkv.so: argument validation, kernel dispatch, error reporting.
 // Every entry point returns a status and never aborts; kernels are only enqueued on the
 // caller's stream (no allocation, no device synchronization) except qkv_device_status.
+#include <limits.h>
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -458,6 +459,7 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
   if (R < 0 || x_rows < 0 || E <= 0 || N <= 0 || K <= 0)
     return fail(QKV_EINVAL, "bad sizes R=%d x_rows=%d E=%d N=%d K=%d", R, x_rows, E, N, K);
   if (K % 64) return fail(QKV_EINVAL, "K %d is not a multiple of 64", K);
+  if (N > INT_MAX - 256) return fail(QKV_EUNSUPPORTED, "at most 2^31 - 257 weight rows (got %d)", N);
   if (act == QKV_ACT_SWIGLU && N % 2)
     return fail(QKV_EINVAL, "N %d is odd: gate and up need as many rows", N);
   if (ldx < K) return fail(QKV_EINVAL, "row stride %lld of x is below K %d", ldx, K);

@@ -152,3 +152,13 @@ def test_experts_layer_refuses_logits_of_other_tokens(x, logits):
                                      (e(4, 128, 8, dt=torch.int32), e(4, 128, 1), e(4, 128, 1)), 2)
     with pytest.raises(ValueError, match="same tokens"):
         layer(e(*x), e(*logits))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch on addresses that are none")
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31 - 256])
+def test_products_refuse_rows_whose_tiles_pass_32_bits(n):
+    lib = _lib.load()
+    far = 1 << 50  # out behind every other range
+    assert _matmul(lib, M=1, N=n, K=64, ldx=64, out=far) == EUNSUP
+    assert _grouped(lib, E=1, N=n, K=64, ldx=64, out=far) == EUNSUP
+    assert _matmul(lib, M=1, N=2 ** 31 - 257, K=64, ldx=64, out=far) == _lib.QKV_ECUDA
