@@ -444,6 +444,12 @@ bool overlap(const void* a, long long na, const void* b, long long nb) {
   return a && b && na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
+// E N K / per bytes, without overflow for sizes that no memory holds
+long long weight_bytes(int E, int N, int K, int per) {
+  const __int128 v = (__int128)E * N * K / per;
+  return v < (1ll << 60) ? (long long)v : 1ll << 60;
+}
+
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Validate and pack the shared arguments of the 4-bit weight products.
@@ -473,6 +479,13 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
     const long long n_out = act == QKV_ACT_SWIGLU ? N / 2 : N;
     if (x_rows > 0 && overlap(x, ((x_rows - 1) * ldx + K) * 2, out, R * n_out * 2))
       return fail(QKV_EINVAL, "out overlaps x");
+    const long long bytes = R * n_out * 2;
+    if (overlap(w, weight_bytes(E, N, K, 2), out, bytes) ||
+        overlap(scales, weight_bytes(E, N, K, 32), out, bytes) ||
+        overlap(biases, weight_bytes(E, N, K, 32), out, bytes))
+      return fail(QKV_EINVAL, "out overlaps the weights");
+    if (overlap(rows, R * 4ll, out, bytes) || overlap(offsets, E * 4ll + 4, out, bytes))
+      return fail(QKV_EINVAL, "out overlaps rows or offsets");
   }
   a = MatmulArgs{};
   a.x = x;
@@ -494,6 +507,10 @@ int setup_matmul(MatmulArgs& a, const void* x, long long ldx, int x_rows, const 
   if (need && (!workspace || ws_bytes < need))
     return fail(QKV_EWORKSPACE, "workspace %zu bytes < required %zu", ws_bytes, need);
   if (need && !aligned16(workspace)) return fail(QKV_EALIGN, "workspace must be 16-byte aligned");
+  const long long n_out = act == QKV_ACT_SWIGLU ? N / 2 : N;
+  if (need && (overlap(workspace, need, out, R * n_out * 2) ||
+               overlap(workspace, need, x, ((x_rows - 1) * ldx + K) * 2)))
+    return fail(QKV_EINVAL, "workspace overlaps x or out");
   a.workspace = workspace;
   a.ws_bytes = ws_bytes;
   a.status = status_ptr();
@@ -577,6 +594,9 @@ int qkv_expert_combine(const void* y, int R, const int* slots, const float* weig
     return fail(QKV_EALIGN, "y, residual and out must be 16-byte aligned");
   const long long bytes = (long long)T * N * 2;
   if (overlap(y, (long long)R * N * 2, out, bytes)) return fail(QKV_EINVAL, "out overlaps y");
+  if (overlap(slots, (long long)T * k * 4, out, bytes) ||
+      overlap(weights, (long long)T * k * 4, out, bytes))
+    return fail(QKV_EINVAL, "out overlaps slots or weights");
   if (residual != out && overlap(residual, bytes, out, bytes))
     return fail(QKV_EINVAL, "out overlaps the residual without being it");
   const int rc = launch_expert_combine(y, R, slots, weights, residual, out, T, k, N, dtype,

@@ -613,7 +613,8 @@ def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, 
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Weighted sum of every token's expert rows: (residual[t] +) sum_j weights[t,j] *
     y[slots[t,j]] for y (R, N), slots int32 and weights fp32 (T, k). Sums in fp32 in j's
-    order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual, not y.
+    order, rounded once to y's dtype; a slot outside y adds nothing. out may be the residual, and
+    is otherwise apart from the inputs.
     """
     idx = y.get_device()
     if (idx < 0 or slots.get_device() != idx or weights.get_device() != idx

@@ -255,9 +255,9 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
  * scales and biases (N, K/64), out (M, N); x, scales, biases and out in `dtype` (bf16 or f16),
  * sums in fp32, one rounding at the end. bits 4, group_size 64, K a multiple of 64, N at most
  * 2^31 - 257. With QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
- * x and w 16-byte aligned, the others naturally; out apart from x. Non-finite x makes its own
- * row of out non-finite (inf or NaN) and no other; so may values above 2^114, whose sums pass
- * the range of fp32. M = 0 does nothing.
+ * x and w 16-byte aligned, the others naturally; out apart from all that is read. Non-finite x
+ * makes its own row of out non-finite (inf or NaN) and no other; so may values above 2^114, whose
+ * sums pass the range of fp32. M = 0 does nothing.
  * workspace: qkv_matmul_workspace_size bytes (0: may be NULL), contents don't matter. R rows
  * of out, E weight matrices (1 here), gathered != 0 when `rows` is given (below).
  */
@@ -304,7 +304,7 @@ int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int norma
 /*
  * out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]]: the experts' rows y (R, N) back
  * in token order, in fp32 and j's order, rounded once. slots (T, k) int32, weights (T, k) fp32,
- * residual (T, N) or NULL, out (T, N) (may be the residual, not y); a slot outside [0, R) adds nothing.
+ * residual (T, N) or NULL, out (T, N) (the residual, or apart from all that is read); a slot outside [0, R) adds nothing.
  */
 int qkv_expert_combine(const void* y, int R, const int* slots, const float* weights,
                        const void* residual, void* out, int T, int k, int N, int dtype,

@@ -162,3 +162,20 @@ def test_products_refuse_rows_whose_tiles_pass_32_bits(n):
     assert _matmul(lib, M=1, N=n, K=64, ldx=64, out=far) == EUNSUP
     assert _grouped(lib, E=1, N=n, K=64, ldx=64, out=far) == EUNSUP
     assert _matmul(lib, M=1, N=2 ** 31 - 257, K=64, ldx=64, out=far) == _lib.QKV_ECUDA
+
+
+@pytest.mark.parametrize("call,over", [
+    # w is 4096 bytes, scales and biases 256 each, of 4 experts four times that; out 256 and 512
+    (_matmul, dict(w=(1 << 20) + 240)), (_matmul, dict(w=(1 << 20) - 4080)),
+    (_matmul, dict(s=(1 << 20) + 254)), (_matmul, dict(b=(1 << 20) - 254)),
+    (_grouped, dict(w=(1 << 20) - 16368)), (_grouped, dict(s=(1 << 20) - 1022)),
+    (_grouped, dict(offsets=(1 << 20) - 16)), (_grouped, dict(rows=(1 << 20) + 508)),
+    (_combine, dict(slots=(1 << 20) + 508)), (_combine, dict(weights=(1 << 20) - 124)),
+    # 2048 x 256 gathered rows: a workspace of 1 MiB
+    (_grouped, dict(R=2048, x_rows=2048, rows=1 << 30, out=1 << 29, N=1024, ws=(1 << 29) + 4194288)),
+    (_grouped, dict(R=2048, x_rows=2048, rows=1 << 30, out=1 << 29, N=1024, ws=16)),
+])
+def test_results_apart_from_all_that_is_read(call, over):
+    lib = _lib.load()
+    assert call(lib, **over) == EINVAL
+    assert b"overlaps" in lib.qkv_last_error()
