@@ -321,12 +321,12 @@ size_t place_smem(int E, int bt) { return (size_t)(2 * E + 1 + (bt + 31) / 32 * 
 // come in the order of the experts, 4 KB at a time.
 //
 // out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]], in fp32, j in order; a slot
-// outside [0, R) adds nothing. VEC values per thread.
+// outside [0, R) adds nothing. VEC values per thread. The result may be the residual: a thread
+// reads its own values before it writes them, and nothing promises that the two are apart.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     expert_combine_kernel(const T* __restrict__ y, int R, const int* __restrict__ slots,
-                          const float* __restrict__ weights, const T* __restrict__ residual,
-                          T* __restrict__ out, long long n_vec, int per_row, int k, int N) {
+                          const float* __restrict__ weights, const T* residual, T* out, long long n_vec, int per_row, int k, int N) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   wait_for_previous();
   if (i >= n_vec) return;
@@ -350,7 +350,12 @@ __global__ void __launch_bounds__(256)
     return make_uint4(__ldg((const uint16_t*)p), 0, 0, 0);
   };
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  const uint4 res = residual ? get(residual + t * N + c) : zero;
+  // (an ordinary load: the residual may be the result, which other threads are writing)
+  uint4 res = zero;
+  if (residual) {
+    if constexpr (VEC == 8) res = *(const uint4*)(residual + t * N + c);
+    else res.x = *(const uint16_t*)(residual + t * N + c);
+  }
 #pragma unroll
   for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
   // eight rows in flight at a time

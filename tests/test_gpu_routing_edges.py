@@ -5,6 +5,9 @@ import subprocess
 import sys
 
 import pytest
+import torch
+
+from chad_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +63,18 @@ ops.expert_combine(y, slots, weights, out=out)
 torch.cuda.synchronize()
 assert bool((out == 2).all())
 """)
+
+
+@pytest.mark.parametrize("t,k,n", [(1, 1, 1), (40, 3, 17), (3000, 2, 33), (700, 8, 264), (5000, 9, 1024)])
+def test_weighted_sum_over_its_residual(t, k, n):
+    """In place and apart are the same bits, at sizes where neighbouring threads share lines."""
+    gen = torch.Generator().manual_seed(t + n)
+    y = torch.randn(t * k, n, generator=gen).half().cuda()
+    slots = torch.randperm(t * k, generator=gen).int().view(t, k).cuda()
+    weights = torch.rand(t, k, generator=gen).cuda()
+    residual = torch.randn(t, n, generator=gen).half().cuda()
+    want = ops.expert_combine(y, slots, weights, residual=residual)
+    for _ in range(4):
+        over = residual.clone()
+        assert ops.expert_combine(y, slots, weights, residual=over, out=over) is over
+        assert torch.equal(over, want)
