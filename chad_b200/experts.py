@@ -19,7 +19,8 @@ from .ops import GROUP_SIZE, QuantTuple
 def quantize_weight(weight: torch.Tensor, bits: int = 4,
                     dtype: Optional[torch.dtype] = None) -> QuantTuple:
     """(w, scales, biases) of a weight (..., N, K), K a multiple of 64: mx.quantize of a weight
-    matrix. The groups run along K, so the rows are quantized as K/64 rows of one group."""
+    matrix. The groups run along K, so the rows are quantized as K/64 rows of one group. (8 bits to
+    store a weight and `ops.dequantize` it; the products take 4.)"""
     *lead, k = weight.shape
     if k % GROUP_SIZE:
         raise ValueError(f"K {k} is not a multiple of {GROUP_SIZE}")

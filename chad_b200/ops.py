@@ -449,8 +449,10 @@ def quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor], bits: int
     w_quant = (w int32 (N, K/8), scales (N, K/64), biases (N, K/64)) in the layout of
     `quantize`, scales and biases in x's dtype (bf16 or fp16). Returns (..., N); with
     activation="swiglu" the first N/2 rows of the weights are the gate and the others the up
-    projection, and silu(gate) * up (..., N/2) comes back. Sums in fp32, one rounding. x may
-    be a 2-D view with a row stride (a multiple of 8 elements).
+    projection, and silu(gate) * up (..., N/2) comes back. Sums in fp32, the result rounded once;
+    with many rows (by the sizes alone) every weight is rounded to x's dtype too, as `dequantize`
+    gives it, so a row's result can differ by that with the number of rows. x may be a 2-D view
+    with a row stride (a multiple of 8 elements). No gradient is recorded.
     """
     # one call per projection per decode step: the host work is kept to plain attribute reads
     w, s, b = w_quant
@@ -508,7 +510,8 @@ def grouped_quantized_matmul(x: torch.Tensor, w_quant: Sequence[torch.Tensor],
     rows offsets[e] .. offsets[e+1] - 1 of the result belong to expert e. Row r of the result
     comes from x[rows[r]] (rows int32 (R,)) or from x[r]. Returns (R, N), or (R, N/2) with
     activation="swiglu"; rows outside [offsets[0], offsets[E]) are not written (of a result
-    allocated here they are undefined). An entry of rows outside x reads a row of zeros.
+    allocated here they are undefined). An entry of rows outside x reads a row of zeros. Rounding
+    as in `quantized_matmul`.
     """
     w, s, b = w_quant
     idx = x.get_device()

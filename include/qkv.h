@@ -253,8 +253,12 @@ int qkv_attention_noalloc(const void* q, const void* kw, const void* ks, const v
  *
  * x (M, K) with ldx elements between rows (a multiple of 8, at least K), w (N, K/8) uint32,
  * scales and biases (N, K/64), out (M, N); x, scales, biases and out in `dtype` (bf16 or f16),
- * sums in fp32, one rounding at the end. bits 4, group_size 64, K a multiple of 64, N at most
- * 2^31 - 257. With QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up of the fp32 sums.
+ * sums in fp32, rounded once at the end. Where many rows share a weight matrix (the sizes alone
+ * decide) every weight is first rounded to `dtype` as well, the value that mx.dequantize gives, so
+ * a row's result can differ by those roundings with the number of rows beside it; where there are
+ * few no weight is rounded. The same call gives the same bits. bits 4, group_size 64, K a multiple
+ * of 64, N at most 2^31 - 257. With QKV_ACT_SWIGLU N is even and out is (M, N/2): silu(gate) * up
+ * of the fp32 sums.
  * x and w 16-byte aligned, the others naturally; out apart from all that is read. Non-finite x
  * makes its own row of out non-finite (inf or NaN) and no other; so may values above 2^114, whose
  * sums pass the range of fp32. M = 0 does nothing.

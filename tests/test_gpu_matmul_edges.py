@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from chad_b200 import ops
-from tests.test_gpu_matmul import check, make_weights, reference, takes_many
+from tests.test_gpu_matmul import check, gate, make_weights, parts64, reference, takes_many
 
 pytestmark = pytest.mark.gpu
 
@@ -79,4 +79,57 @@ def test_experts_with_fewer_rows_to_a_pass(k):
     for i, (a, b) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:])):
         if a < b:
             want, err = reference(x[a:b], [t[i] for t in wq], None, torch.bfloat16)
+            check(got[a:b], want, err, f"expert {i}")
+
+
+def reference_of_few_rows(x, wq, act, dtype):
+    """(y, allowed error) where no weight is rounded: the terms of `reference` but for that one.
+
+    Also y of weights rounded to dtype, from the oracle, which the bound can tell apart up to a K of
+    about 2048 (past that the sums' own terms are larger).
+    """
+    c, s, b = parts64(*wq)
+    xd, wd, eps = x.double(), s * c + b, torch.finfo(dtype).eps / 2
+    y, rounded = xd @ wd.t(), xd @ wd.to(dtype).double().t()
+    zero = 128 if dtype is torch.bfloat16 else 0  # a code enters the MMA as zero + code
+    mag = xd.abs() @ (s.abs() * (zero + c) + (b - zero * s).abs()).t()
+    err = 2.0 ** -20 * mag + (x.shape[1] // 64) * 2.0 ** -23 * (xd.abs() @ wd.abs().t())
+    if act:
+        g, u = y.chunk(2, -1)
+        eg, eu = err.chunk(2, -1)
+        silu = g / (1 + torch.exp(-g))
+        y, err = silu * u, 1.1 * eg * (u.abs() + eu) + silu.abs() * eu
+        err = err + 2.0 ** -21 * y.abs()
+        rounded = gate(rounded)
+    return y, err + eps * (y.abs() + err) + torch.finfo(dtype).smallest_normal * eps, rounded
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 64), (1, 515, 2048), (3, 1000, 4096), (8, 260, 1088), (16, 130, 2048),
+                                   (40, 100, 192), (48, 90, 4096), (2, 60, 20480)])
+@pytest.mark.parametrize("act", [None, "swiglu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_round_no_weight(m, n, k, act, dtype):
+    n += n % 2 if act else 0
+    assert not takes_many(m, 1, n, k)
+    gen = torch.Generator().manual_seed(m + n + k)
+    wq = make_weights(gen, (n,), k, dtype)
+    x = torch.randn(m, k, generator=gen).to(dtype).cuda()
+    want, err, rounded = reference_of_few_rows(x, wq, act, dtype)
+    assert k > 2048 or bool(((rounded - want).abs() > err).any())
+    check(ops.quantized_matmul(x, wq, activation=act), want, err, f"{m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("act", [None, "swiglu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_of_experts_round_no_weight(act, dtype):
+    gen = torch.Generator().manual_seed(21)
+    counts, n, k = [3, 0, 9, 1, 8], 200, 1088
+    assert not takes_many(sum(counts), len(counts), n, k)
+    wq = make_weights(gen, (len(counts), n), k, dtype)
+    offsets = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    x = torch.randn(sum(counts), k, generator=gen).to(dtype).cuda()
+    got = ops.grouped_quantized_matmul(x, wq, offsets, activation=act)
+    for i, (a, b) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:])):
+        if a < b:
+            want, err, _ = reference_of_few_rows(x[a:b], [t[i] for t in wq], act, dtype)
             check(got[a:b], want, err, f"expert {i}")
