@@ -78,3 +78,34 @@ def test_weighted_sum_over_its_residual(t, k, n):
         over = residual.clone()
         assert ops.expert_combine(y, slots, weights, residual=over, out=over) is over
         assert torch.equal(over, want)
+
+
+def test_first_calls_of_a_process_are_captured():
+    """Shared-memory bounds, module loading and the status word need no call outside the capture."""
+    fresh("""
+import torch
+from chad_b200 import ops
+gen = torch.Generator().manual_seed(1)
+def weights(*lead, k):
+    return (torch.randint(-2 ** 31, 2 ** 31, (*lead, k // 8), generator=gen).int().cuda(),
+            torch.rand(*lead, k // 64, generator=gen).bfloat16().cuda(),
+            torch.randn(*lead, k // 64, generator=gen).bfloat16().cuda())
+few, many = weights(4, 64, k=128), weights(4, 1000, k=512)
+x, y = torch.randn(3, 128, generator=gen).bfloat16().cuda(), torch.randn(700, 512, generator=gen).bfloat16().cuda()
+logits = torch.randn(700, 4, generator=gen).cuda()
+def calls():
+    r = ops.route_topk(logits, 2)
+    return [ops.quantized_matmul(x, [t[0] for t in few]), ops.quantized_matmul(y, [t[0] for t in many]),
+            *r, ops.grouped_quantized_matmul(y, many, r.offsets, rows=r.rows, activation="swiglu"),
+            ops.expert_combine(torch.cat([y, y]), r.slots, r.weights, residual=y)]
+graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+stream.wait_stream(torch.cuda.current_stream())
+torch.cat([y, y])
+torch.cuda.synchronize()
+with torch.cuda.graph(graph, stream=stream):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, calls()):
+    assert torch.equal(a, b)
+""")
