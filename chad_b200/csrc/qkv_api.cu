@@ -589,9 +589,10 @@ int qkv_expert_combine(const void* y, int R, const int* slots, const float* weig
     return fail(QKV_EINVAL, "bad sizes R=%d T=%d k=%d N=%d", R, T, k, N);
   if (T == 0) return QKV_OK;
   if ((R > 0 && !y) || !slots || !weights || !out) return fail(QKV_EINVAL, "null pointer");
-  if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned(slots, 4) ||
+  const size_t row = N % 8 ? 2 : 16;  // rows of whole vectors are read as vectors
+  if (!aligned(y, row) || !aligned(residual, row) || !aligned(out, row) || !aligned(slots, 4) ||
       !aligned(weights, 4))
-    return fail(QKV_EALIGN, "y, residual and out must be 16-byte aligned");
+    return fail(QKV_EALIGN, "y, residual and out must be %zu-byte aligned", row);
   const long long bytes = (long long)T * N * 2;
   if (overlap(y, (long long)R * N * 2, out, bytes)) return fail(QKV_EINVAL, "out overlaps y");
   if (overlap(slots, (long long)T * k * 4, out, bytes) ||

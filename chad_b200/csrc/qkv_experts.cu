@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 int launch_combine_t(const void* y, int R, const int* slots, const float* weights,
                      const void* residual, void* out, int tokens, int k, int N, cudaStream_t st) {
-  const bool vec = N % 8 == 0;
+  const bool vec = N % 8 == 0;  // (y, residual and out are then 16-byte aligned)
   const int per_row = vec ? N / 8 : N;
   const long long n = (long long)tokens * per_row;
   const long long blocks = (n + 255) / 256;

@@ -308,7 +308,8 @@ int qkv_route_topk(const void* logits, int dtype, int T, int E, int k, int norma
 /*
  * out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]]: the experts' rows y (R, N) back
  * in token order, in fp32 and j's order, rounded once. slots (T, k) int32, weights (T, k) fp32,
- * residual (T, N) or NULL, out (T, N) (the residual, or apart from all that is read); a slot outside [0, R) adds nothing.
+ * residual (T, N) or NULL, out (T, N) (the residual, or apart from all that is read); y, residual
+ * and out 16-byte aligned, where N is no multiple of 8 naturally; a slot outside [0, R) adds nothing.
  */
 int qkv_expert_combine(const void* y, int R, const int* slots, const float* weights,
                        const void* residual, void* out, int T, int k, int N, int dtype,

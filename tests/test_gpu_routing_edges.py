@@ -109,3 +109,14 @@ torch.cuda.synchronize()
 for a, b in zip(got, calls()):
     assert torch.equal(a, b)
 """)
+
+
+def test_weighted_sum_of_slices_with_odd_rows():
+    gen = torch.Generator().manual_seed(5)
+    pool = torch.randn(30, 17, generator=gen).bfloat16().cuda()
+    y, residual, out = pool[1:13], pool[13:17], torch.zeros(6, 17, dtype=torch.bfloat16, device="cuda")
+    slots = torch.randperm(12, generator=gen).int().view(4, 3).cuda()
+    weights = torch.rand(4, 3, generator=gen).cuda()
+    ops.expert_combine(y, slots, weights, residual=residual, out=out[1:5])
+    assert torch.equal(out[1:5], ops.expert_combine(y.clone(), slots, weights, residual=residual.clone()))
+    assert bool((out[[0, 5]] == 0).all())

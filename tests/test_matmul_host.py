@@ -179,3 +179,12 @@ def test_results_apart_from_all_that_is_read(call, over):
     lib = _lib.load()
     assert call(lib, **over) == EINVAL
     assert b"overlaps" in lib.qkv_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch on addresses that are none")
+def test_combine_asks_for_vectors_only_where_rows_are_whole_ones():
+    lib = _lib.load()
+    odd = dict(N=63, y=34, out=(1 << 20) + 2)
+    assert _combine(lib, **odd, residual=(1 << 21) + 6) == _lib.QKV_ECUDA
+    assert _combine(lib, **(odd | dict(y=33))) == EALIGN
+    assert _combine(lib, **(odd | dict(N=64))) == EALIGN
