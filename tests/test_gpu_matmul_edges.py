@@ -133,3 +133,21 @@ def test_few_rows_of_experts_round_no_weight(act, dtype):
         if a < b:
             want, err, _ = reference_of_few_rows(x[a:b], [t[i] for t in wq], act, dtype)
             check(got[a:b], want, err, f"expert {i}")
+
+
+@pytest.mark.parametrize("m", [1, 9, 2000])
+@pytest.mark.parametrize("k", [192, 512, 1024])
+def test_scales_that_begin_anywhere(m, k):
+    """Scales and biases from an odd place of a larger tensor, for every way that they are copied."""
+    gen = torch.Generator().manual_seed(m + k)
+    n = 1000
+    assert takes_many(m, 1, n, k) == (m == 2000)
+    w, s, b = make_weights(gen, (n,), k, torch.bfloat16)
+    x = torch.randn(m, k, generator=gen).bfloat16().cuda()
+    want = ops.quantized_matmul(x, (w, s, b))
+    for off_s, off_b in ((1, 1), (2, 4), (4, 0), (8, 3)):
+        views = []
+        for t, off in ((s, off_s), (b, off_b)):
+            pool = torch.full((t.numel() + 16,), float("nan"), dtype=t.dtype, device="cuda")
+            views.append(pool[off:off + t.numel()].view(t.shape).copy_(t))
+        assert torch.equal(ops.quantized_matmul(x, (w, *views)), want)
