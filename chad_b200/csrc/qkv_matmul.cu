@@ -20,11 +20,13 @@
 // a clock, and fragments read from global memory directly cost it 8 lines per 256 bytes. Warps
 // of a CTA split K until the machine has enough of them to keep HBM busy, and add their sums
 // through shared memory in a fixed order. The rows of x stay in shared memory, already paired.
-// One row through 131071x2048 (f16): 31.4 us, 4.8 of 6.6 TB/s; a chunk of 4096 weights takes about
-// 290 instructions of a warp, two thirds of them the codes' masks and shifts (ALU, every other
-// clock), so the SMs issue for most of that time. Few weights are bound by latency: one row
-// through 5120x2048 5.1 us, of which a launch, the wait for x and one chunk's trip are 4. Three
-// CTAs per SM with 80 registers were no faster (32.4 and 5.5 us).
+// One row through 131071x2048 (f16): 31 us, 4.9 of 6.6 TB/s; a chunk of 4096 weights takes about
+// 290 instructions of a warp, 112 of them the codes' masks and shifts. No unit is full (issue 59%
+// of clocks, ALU pipe 57%, HBM 4.5 TB/s under the profiler): of the 6 clocks between two
+// instructions of a warp 1.2 go to another warp's turn, 1.1 to fixed latencies, 0.9 to the ALU
+// pipe's and 0.3 to a load, so fewer instructions, not more loads in flight, would shorten it. Few
+// weights are bound by latency: one row through 5120x2048 5.0 us, of which a launch, the wait for
+// x and one chunk's trip are 4. Three CTAs per SM with 80 registers were no faster (32.4 and 5.5).
 #include <algorithm>
 #include <atomic>
 

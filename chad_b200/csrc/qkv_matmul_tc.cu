@@ -25,13 +25,16 @@
 // multiply-add, the value mx.dequantize gives; sums are fp32. The kernel for few rows rounds no
 // weight: relative to the exact product the results are off by 2.2e-3 (bf16, the output's own
 // rounding included) against its 1.7e-3, of a gated product by 2.7e-3 against 1.7e-3; in f16 by
-// 2.8e-4 and 3.4e-4 against 2.1e-4. Weights in two terms would double the MMAs and the stores.
+// 2.8e-4 and 3.4e-4 against 2.1e-4. A choice, which the documents of the calls state: weights in
+// two terms need twice the MMAs, and those alone take 2048 rows through 5120x2048 from 32.6 to 54.6
+// us, 16384 expert rows from 143 to 210 and 1332 from 39 to 53 (measured with every MMA issued
+// twice), for an error that stays below the result's own rounding in all but the gated products.
 //
-// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 141 us: the tensor pipe is
+// What bounds it, measured: 128 experts of 1536x2048 at 16384 rows, 143 us: the tensor pipe is
 // busy 47% of the time, the ALU pipe with dequantizing 52% (its warps wait for
 // freed A stages about as often as the MMAs wait for full ones), HBM at 1.8 TB/s. 2048 rows through
-// 5120x2048: 32.7 us, 1310 TFLOP/s, tensor pipe 62 to 76%. Run without a pause both are at the
-// card's power limit (1540 MHz): 160 and 39 us.
+// 5120x2048: 32.6 us, 1320 TFLOP/s, tensor pipe 62 to 76%. Run without a pause both are at the
+// card's power limit (1540 MHz): 168 and 40 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -148,7 +151,7 @@ __device__ __forceinline__ uint32_t elect_one() {
 // A value that all lanes have, in a uniform register. The loops that issue MMAs and copies count
 // to such values and call no function (which would not preserve the registers): their operands
 // then stay in uniform registers, instead of being moved there for every instruction (16384
-// expert rows 146 us with loops that the compiler takes for divergent, 141 so).
+// expert rows 3% slower with loops that the compiler takes for divergent).
 __device__ __forceinline__ uint32_t uniform(uint32_t v) {
   return __reduce_max_sync(0xffffffffu, v);
 }
