@@ -326,7 +326,8 @@ size_t place_smem(int E, int bt) { return (size_t)(2 * E + 1 + (bt + 31) / 32 * 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     expert_combine_kernel(const T* __restrict__ y, int R, const int* __restrict__ slots,
-                          const float* __restrict__ weights, const T* residual, T* out, long long n_vec, int per_row, int k, int N) {
+                          const float* __restrict__ weights, const T* residual, T* out,
+                          long long n_vec, int per_row, int k, int N) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   wait_for_previous();
   if (i >= n_vec) return;

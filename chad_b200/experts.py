@@ -3,7 +3,8 @@
 The reference runs its models with weights in the same affine format as the cache
 (tests/test_engine_kvquant.py:22-37): every projection is an mx.quantized_matmul, and its
 mixture-of-experts layers are fused kernels over stacked quantized experts
-(src/chad/mlx_moe_fused.py). Both are built here on the operators of `ops`.
+(src/chad/mlx_moe_fused.py). Both are built here on the operators of `ops`, forward only: like
+the attention, none of them records a gradient.
 """
 
 from __future__ import annotations
